@@ -6993,7 +6993,9 @@ struct AdamwArgs {
     float decay, w1, b2, w2, eps, neg_step_size, bc2_sqrt;
 };
 
+// Products and sums round one by one, as torch's separate operations do; the second moment alone is fused.
 __global__ void __launch_bounds__(256) adamw_kernel(const AdamwArgs a) {
+#pragma clang fp contract(off)
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.n) return;
     int lo = 0, hi = a.n_tensors;                                  // starts[lo] <= i < starts[hi]
@@ -7006,8 +7008,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(const AdamwArgs a) {
     float p = a.p[lo][o], m = a.m[lo][o], v = a.v[lo][o];
     p *= a.decay;
     m = m + (g - m) * a.w1;
-    v = v * a.b2;
-    v = v + (a.w2 * g) * g;
+    v = __builtin_fmaf(a.w2 * g, g, v * a.b2);
     const float denom = sqrtf(v) / a.bc2_sqrt + a.eps;
     p = p + a.neg_step_size * (m / denom);
     a.p[lo][o] = p; a.m[lo][o] = m; a.v[lo][o] = v;
