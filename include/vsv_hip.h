@@ -576,6 +576,98 @@ int vsv_adamw_step(void *const *params, void *const *exp_avg, void *const *exp_a
 int vsv_dropout_mask(float p, uint64_t seed, int id, int layer, long n_rows, int T, int hidden,
                      float *out, void *stream);
 
+/* ---- sequence memory: short causal convolution and selective scan ----------------------------------------
+ * A memory beside the LSTM / GRU / RNN ones (the nn.LSTM(batch_first) call sites :155, :307, :476 are what it can stand in
+ * for); the reference has none of this kind.  Sequences are (B, T, D) tensors of `dtype` whose features are contiguous and
+ * whose sequence and time strides (in elements) are free; outputs are contiguous; weights, states and their gradients are
+ * contiguous float32.  `lengths` (B int32, device, may be NULL): rows [lengths[b], T) are padding -- never read, their
+ * outputs and gradients are zero, the state stops at the length; values outside [0, T] count as the nearest of the two. */
+#define VSV_F32 0
+#define VSV_BF16 1
+#define VSV_F16 2
+#define VSV_CONV_MAX_TAPS 4
+#define VSV_SSM_MAX_STATE 16
+
+/* y[t] = act(bias + sum_k w[:, k] xs[t - K + 1 + k]), xs = state_in's K - 1 rows followed by x; act = silu or nothing.
+ * state_out (B, K-1, D) = the last K - 1 rows of xs.  Of vsv_short_conv_step state_out is read and written in place
+ * (x, y: (B, D), state_in, lengths and T unused). */
+typedef struct vsv_short_conv_desc {
+    int dtype, K, silu;
+    long B, T, D;
+    const void *x;  long x_bs, x_ts;
+    const float *w;                         /* (D, K) */
+    const float *bias;                      /* (D) or NULL */
+    const float *state_in;                  /* (B, K-1, D) or NULL = zeros */
+    const int *lengths;
+    void *y;                                /* (B, T, D) */
+    float *state_out;                       /* or NULL */
+} vsv_short_conv_desc;
+typedef struct vsv_short_conv_grads {
+    const void *dy;  long dy_bs, dy_ts;
+    const float *d_state_out;               /* (B, K-1, D) or NULL */
+    void *dx;                               /* (B, T, D) */
+    float *dw, *dbias, *d_state_in;         /* each may be NULL */
+} vsv_short_conv_grads;
+int vsv_short_conv(const vsv_short_conv_desc *a, void *stream);
+size_t vsv_short_conv_backward_ws_bytes(const vsv_short_conv_desc *a);
+int vsv_short_conv_backward(const vsv_short_conv_desc *a, const vsv_short_conv_grads *g, void *ws, size_t ws_bytes,
+                            void *stream);
+int vsv_short_conv_step(const vsv_short_conv_desc *a, void *stream);
+
+/* delta = softplus(dt + dt_bias) (softplus = 0: without it);  h_t = exp(delta a) h_{t-1} + delta x b_t;
+ * y_t = (c_t . h_t + skip x_t) silu(gate_t).  a (D, N); h (B, D, N); b, c (B, T, G, N), channel d in group d / (D / G).
+ * saved (vsv_ssm_saved_floats, may be NULL): filled by vsv_ssm_scan for vsv_ssm_scan_backward, which gets the same
+ * descriptor.  Of vsv_ssm_step state_out is read and written in place (x, dt, gate, y: (B, D), b, c: (B, G, N); T, state_in,
+ * lengths and saved unused). */
+typedef struct vsv_ssm_desc {
+    int dtype, N, softplus;
+    long B, T, D, G;
+    const void *x;  long x_bs, x_ts;
+    const void *dt;  long dt_bs, dt_ts;
+    const void *gate;  long gate_bs, gate_ts;         /* or NULL */
+    const void *b;  long b_bs, b_ts, b_gs;
+    const void *c;  long c_bs, c_ts, c_gs;
+    const float *a, *skip, *dt_bias;                  /* skip, dt_bias may be NULL */
+    const float *state_in;                            /* or NULL = zeros */
+    const int *lengths;
+    void *y;
+    float *state_out;                                 /* or NULL */
+    float *saved;
+} vsv_ssm_desc;
+typedef struct vsv_ssm_grads {
+    const void *dy;  long dy_bs, dy_ts;
+    const float *d_state_out;                         /* or NULL */
+    void *dx, *ddt, *dgate;                           /* (B, T, D); dgate with a gate only */
+    void *db, *dc;                                    /* (B, T, G, N) */
+    float *da, *dskip, *ddt_bias, *d_state_in;        /* each may be NULL */
+} vsv_ssm_grads;
+size_t vsv_ssm_saved_floats(const vsv_ssm_desc *a);
+size_t vsv_ssm_scan_ws_bytes(const vsv_ssm_desc *a);
+int vsv_ssm_scan(const vsv_ssm_desc *a, void *ws, size_t ws_bytes, void *stream);
+size_t vsv_ssm_scan_backward_ws_bytes(const vsv_ssm_desc *a);
+int vsv_ssm_scan_backward(const vsv_ssm_desc *a, const vsv_ssm_grads *g, void *ws, size_t ws_bytes, void *stream);
+int vsv_ssm_step(const vsv_ssm_desc *a, void *stream);
+
+/* ---- AdamW over many tensors, moments in 32 or 8 bits ------------------------------------------------------
+ * The optimizer step of vsv_adamw_step for tensors with gradients of their own, in float32, bfloat16 or float16 (`dtype`
+ * of p and g).  `tensors` is a HOST array; its contents travel in the launches' arguments (60 tensors each).
+ * bits = 32: m, v float32.  bits = 8: m int8, v uint8 codes with a float32 scale of each per VSV_ADAMW_BLOCK elements
+ * (m = sign s (k/127)^2, v = s (k/255)^4, to float32).  All state starts as zeros; step = the count after this step (>= 1).
+ * vsv_adamw_read8: p and g of an entry are two float32 outputs and receive the values m and v stand for. */
+#define VSV_ADAMW_BLOCK 256
+#define VSV_ADAMW_WEYL_I 0xC13FA9A9u                  /* the dither's steps per element and per step: 2^32 / 1.32472, / 1.75488 */
+#define VSV_ADAMW_WEYL_T 0x91E10DA5u
+typedef struct vsv_adamw_tensor {
+    void *p;
+    const void *g;
+    void *m, *v;
+    float *m_scale, *v_scale;               /* bits = 8 */
+    long n;
+} vsv_adamw_tensor;
+int vsv_adamw_multi(const vsv_adamw_tensor *tensors, int n_tensors, int dtype, int bits, double lr, double beta1, double beta2,
+                    double eps, double weight_decay, long step, void *stream);
+int vsv_adamw_read8(const vsv_adamw_tensor *tensors, int n_tensors, void *stream);
+
 /* ---- profiling aid -----------------------------------------------------------------
  * Arms the NEXT vsv_decode call made by this thread: it records the two hipEvent_t
  * (created by the caller with timing enabled) on the call's stream immediately before

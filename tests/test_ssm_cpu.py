@@ -1,0 +1,161 @@
+"""vsv.ssm and vsv.optim without a GPU: the references' gradients against differences, and every refusal."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ssm_reference import conv_ref, scan_ref
+
+
+def _case(seed, B=2, T=5, D=4, N=3, G=2, K=3):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)        # noqa: E731
+    scan = dict(x=r(B, T, D), dt=r(B, T, D), a=-torch.rand(D, N, generator=g, dtype=torch.float64) - 0.2, b=r(B, T, G, N), c=r(B, T, G, N),
+                skip=r(D), gate=r(B, T, D), dt_bias=r(D), h0=r(B, D, N))
+    conv = dict(x=r(B, T, D), w=r(D, K), bias=r(D), h0=r(B, K - 1, D))
+    return scan, conv, r(B, T, D), r(B, D, N), r(B, K - 1, D)
+
+
+@pytest.mark.parametrize("lengths", [None, [5, 0], [3, 1]])
+@pytest.mark.parametrize("flag", [True, False])
+def test_reference_gradients_are_the_differences(lengths, flag):
+    """Each formula's gradient along a random direction against a central difference of the plain forward: the difference's
+    own error is h^2 / 6 of a third derivative, 1e-10 at h = 1e-5, and rounding 1e-16 / h = 1e-11, of values around 10."""
+    scan, conv, dy, dh, dc = _case(1)
+    h = 1e-5
+    loss = lambda o, d: (o["y"] * dy).sum() + (o["state"] * d).sum()        # noqa: E731
+    for args, ref, d in ((scan, scan_ref, dh), (conv, conv_ref, dc)):
+        got = ref(*args.values(), lengths, flag, dy, d)
+        for name, t in args.items():
+            v = torch.randn(t.shape, generator=torch.Generator().manual_seed(7), dtype=torch.float64)
+            plus = loss(ref(*{**args, name: t + h * v}.values(), lengths, flag), d)
+            minus = loss(ref(*{**args, name: t - h * v}.values(), lengths, flag), d)
+            slope = ((plus - minus) / (2 * h)).item()
+            assert abs(slope - (got[name] * v).sum().item()) <= 1e-7 * (1 + abs(slope)), name
+
+
+def _scan_tensors(B=2, T=4, D=6, N=4, G=1, dtype=torch.float32):
+    z = torch.zeros
+    return dict(x=z(B, T, D, dtype=dtype), dt=z(B, T, D, dtype=dtype), a=z(D, N), b=z(B, T, G, N, dtype=dtype), c=z(B, T, G, N, dtype=dtype))
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(x=torch.zeros(4, 6)), "x must be"),
+    (dict(x=torch.zeros(2, 4, 6, dtype=torch.float64)), "x must be"),
+    (dict(dt=torch.zeros(2, 4, 6, dtype=torch.bfloat16)), "dt must be"),
+    (dict(dt=torch.zeros(2, 5, 6)), "dt must be"),
+    (dict(a=torch.zeros(6, 17)), "a must be"),
+    (dict(a=torch.zeros(6, 0)), "a must be"),
+    (dict(a=torch.zeros(5, 4)), "a must be"),
+    (dict(a=torch.zeros(6, 4, dtype=torch.bfloat16)), "a must be"),
+    (dict(b=torch.zeros(2, 4, 4, 4)), "b must be"),
+    (dict(b=torch.zeros(2, 4, 2, 4)), "groups"),
+    (dict(c=torch.zeros(2, 4, 1, 5)), "c must be"),
+    (dict(skip=torch.zeros(5)), "skip must be"),
+    (dict(gate=torch.zeros(2, 4, 5)), "gate must be"),
+    (dict(dt_bias=torch.zeros(6, dtype=torch.float64)), "dt_bias must be"),
+    (dict(initial_state=torch.zeros(2, 6, 3)), "initial_state must be"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths must be"),
+    (dict(lengths=torch.zeros(2)), "lengths must be"),
+    (dict(lengths=[1, 2]), "lengths must be"),
+])
+def test_scan_refuses(change, word):
+    from vsv.ssm import ssm_scan
+    with pytest.raises(ValueError, match=word):
+        ssm_scan(**{**_scan_tensors(), **change})
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(x=torch.zeros(2, 4)), "x must be"),
+    (dict(x=torch.zeros(2, 4, 6, dtype=torch.int32)), "x must be"),
+    (dict(weight=torch.zeros(6, 5)), "weight must be"),
+    (dict(weight=torch.zeros(5, 4)), "weight must be"),
+    (dict(weight=torch.zeros(6, 4, dtype=torch.float16)), "weight must be"),
+    (dict(bias=torch.zeros(5)), "bias must be"),
+    (dict(initial_state=torch.zeros(2, 4, 6)), "initial_state must be"),
+])
+def test_conv_refuses(change, word):
+    from vsv.ssm import short_conv
+    with pytest.raises(ValueError, match=word):
+        short_conv(**{**dict(x=torch.zeros(2, 4, 6), weight=torch.zeros(6, 4)), **change})
+
+
+def test_steps_refuse():
+    from vsv.ssm import short_conv_step, ssm_step
+    x, w = torch.zeros(3, 6), torch.zeros(6, 4)
+    a, b = torch.zeros(6, 4), torch.zeros(3, 4)
+    for state in (torch.zeros(3, 3, 6, dtype=torch.float64), torch.zeros(3, 4, 6), torch.zeros(3, 6, 3).transpose(1, 2),
+                  torch.zeros(1, 3, 6).expand(3, 3, 6)):
+        with pytest.raises(ValueError, match="state must be"):
+            short_conv_step(x, state, w)
+    for state in (None, torch.zeros(3, 4, 6), torch.zeros(1, 6, 4).expand(3, 6, 4), torch.zeros(3, 6, 8)[:, :, ::2]):
+        with pytest.raises(ValueError, match="state must be"):
+            ssm_step(x, x, a, b, b, state=state)
+    with pytest.raises(ValueError, match="b must be"):
+        ssm_step(x, x, a, torch.zeros(2, 4), b, state=torch.zeros(3, 6, 4))
+
+
+def test_no_cpu_fallback():
+    from vsv.optim import AdamW
+    from vsv.ssm import short_conv, short_conv_step, ssm_scan, ssm_step
+    t = _scan_tensors()
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+    for call in (lambda: ssm_scan(**t), lambda: short_conv(t["x"], torch.zeros(6, 2)),
+                 lambda: short_conv_step(torch.zeros(2, 6), torch.zeros(2, 1, 6), torch.zeros(6, 2)),
+                 lambda: ssm_step(t["x"][:, 0], t["dt"][:, 0], t["a"], t["b"][:, 0], t["c"][:, 0], state=torch.zeros(2, 6, 4)),
+                 lambda: AdamW([p]).step()):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
+
+
+def test_optimizer_refuses():
+    from vsv.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4, 3))
+    for bad in (dict(state_bits=4), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(weight_decay=-0.1),
+                dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            AdamW([p], **bad)
+    for q in (torch.zeros(4, dtype=torch.float64), torch.zeros(4, 3).t()):
+        with pytest.raises(ValueError):
+            AdamW([torch.nn.Parameter(q)])
+    opt = AdamW([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2, dtype=torch.float64))]})
+    assert len(opt.param_groups) == 1
+    p.grad = torch.zeros(4, 3).to_sparse()
+    with pytest.raises(ValueError, match="gradient"):
+        opt.step()
+    with pytest.raises(ValueError, match="8 bits"):
+        AdamW([p], state_bits=8).load_state_dict({"state": {0: {"step": 1, "exp_avg": torch.zeros(4, 3)}}, "param_groups": opt.state_dict()["param_groups"]})
+
+
+def test_c_entries_check_their_arguments():
+    from vsv import lib as vlib
+    L = vlib.load()
+    conv = lambda **k: vlib.VsvShortConv(**{**dict(dtype=0, K=4, silu=1, B=1, T=4, D=8, x=16, x_bs=32, x_ts=8, w=16, y=16), **k})    # noqa: E731
+    scan = lambda **k: vlib.VsvSsm(**{**dict(dtype=0, N=4, softplus=1, B=1, T=4, D=8, G=1, x=16, dt=16, b=16, c=16, a=16, y=16), **k})   # noqa: E731
+    for bad in (conv(K=0), conv(K=5), conv(B=-1), conv(T=-1), conv(D=0), conv(dtype=3), conv(w=None), conv(x=None), conv(y=None)):
+        assert L.vsv_short_conv(C.byref(bad), None) == -1 and L.vsv_last_error()
+        assert L.vsv_short_conv_backward(C.byref(bad), None, None, 0, None) == -1
+    assert L.vsv_short_conv(None, None) == -1
+    g = vlib.VsvShortConvGrads(dy=16, dx=16)
+    assert L.vsv_short_conv_backward(C.byref(conv()), C.byref(g), None, 0, None) == -1 and b"workspace" in L.vsv_last_error()
+    assert L.vsv_short_conv_step(C.byref(conv()), None) == -1                                  # (no state)
+    for bad in (scan(N=0), scan(N=17), scan(G=3), scan(G=0), scan(B=-1), scan(T=-1), scan(D=0), scan(dtype=-1), scan(a=None), scan(x=None),
+                scan(c=None), scan(y=None)):
+        assert L.vsv_ssm_scan(C.byref(bad), None, 0, None) == -1 and L.vsv_last_error()
+        assert L.vsv_ssm_scan_backward(C.byref(bad), None, None, 0, None) == -1
+    s = vlib.VsvSsmGrads(dy=16, dx=16, ddt=16, db=16, dc=16)
+    assert L.vsv_ssm_scan_backward(C.byref(scan()), C.byref(s), 16, 1 << 30, None) == -1       # (nothing saved)
+    assert L.vsv_ssm_scan_backward(C.byref(scan(saved=16)), C.byref(s), None, 0, None) == -1 and b"workspace" in L.vsv_last_error()
+    assert L.vsv_ssm_step(C.byref(scan()), None) == -1                                         # (no state)
+    row = (C.c_uint64 * 7)(16, 16, 16, 16, 0, 0, 4)
+    ok = (1e-3, 0.9, 0.999, 1e-8, 0.01, 1)
+    for bits, hyper in ((16, ok), (8, ok), (32, (-1.0,) + ok[1:]), (32, ok[:1] + (1.0,) + ok[2:]), (32, ok[:5] + (0,)), (32, (float("nan"),) + ok[1:])):
+        assert L.vsv_adamw_multi(row, 1, 0, bits, *hyper, None) == -1, (bits, hyper)
+    assert L.vsv_adamw_multi(row, 1, 3, 32, *ok, None) == -1
+    assert L.vsv_adamw_multi(None, 1, 0, 32, *ok, None) == -1
+    assert L.vsv_adamw_multi((C.c_uint64 * 7)(0, 16, 16, 16, 0, 0, 4), 1, 0, 32, *ok, None) == -1
+    assert L.vsv_adamw_read8(row, 1, None) == -1
+    assert L.vsv_adamw_multi(None, 0, 0, 32, *ok, None) == 0                                   # nothing to do

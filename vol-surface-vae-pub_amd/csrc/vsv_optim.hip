@@ -1,0 +1,261 @@
+// AdamW over many tensors in one launch, moments held in 32 bits or in 8.
+//   p *= 1 - lr wd;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+//   p -= lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// Every value is read once and written once and little is computed: bound by memory.  The tensors' addresses travel in
+// the launch's arguments, so there is no table in device memory to keep or to copy, and nothing to look up on replay.
+#include <cfloat>
+#include <cmath>
+
+#include "vsv_ops.h"
+
+namespace vsv {
+namespace {
+
+constexpr int kMaxTensors = 60;      // per launch: the argument block stays below 4 KiB
+constexpr int kBlock8 = VSV_ADAMW_BLOCK;
+
+struct Hyper {
+    float decay, b1, w1, b2, w2, eps, rate, root;
+    double b1d, w1d, b2d, w2d;
+    unsigned dither;
+};
+struct Table {
+    vsv_adamw_tensor t[kMaxTensors];
+    unsigned first[kMaxTensors + 1]; // first workgroup of each tensor
+    int n;
+};
+
+__device__ inline int tensor_of(const Table& tab, unsigned blk) {
+    int lo = 0, hi = tab.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tab.first[mid] <= blk) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// ---- 32 bits -----------------------------------------------------------------------------------------------------
+constexpr int kPer32 = 4, kIter32 = 2, kChunk32 = 256 * kPer32 * kIter32;
+
+__device__ inline void update32(float& p, float g, float& m, float& v, const Hyper& h) {
+    m = __builtin_fmaf(h.b1, m, h.w1 * g);
+    v = __builtin_fmaf(h.b2, v, h.w2 * g * g);
+    p = p * h.decay - h.rate * m / (sqrtf(v) / h.root + h.eps);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) adamw32_kernel(const Table tab, const Hyper h) {
+    const int ti = tensor_of(tab, blockIdx.x);
+    const vsv_adamw_tensor& e = tab.t[ti];
+    const long base = (long)(blockIdx.x - tab.first[ti]) * kChunk32;
+    T* p = (T*)e.p; const T* g = (const T*)e.g; float *m = (float*)e.m, *v = (float*)e.v;
+    const bool wide = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0;
+    if (wide && base + kChunk32 <= e.n) {
+        float pv[kIter32][4], gv[kIter32][4], mv[kIter32][4], vv[kIter32][4];
+#pragma unroll
+        for (int i = 0; i < kIter32; ++i) {
+            const long o = base + (i * 256 + threadIdx.x) * 4;
+            load_vec<T, 4>(p + o, pv[i]); load_vec<T, 4>(g + o, gv[i]);
+            load_vec<float, 4>(m + o, mv[i]); load_vec<float, 4>(v + o, vv[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kIter32; ++i) {
+            const long o = base + (i * 256 + threadIdx.x) * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) update32(pv[i][j], gv[i][j], mv[i][j], vv[i][j], h);
+            store_vec<T, 4>(p + o, pv[i]);
+            store_vec<float, 4>(m + o, mv[i]); store_vec<float, 4>(v + o, vv[i]);
+        }
+        return;
+    }
+    for (long o = base + threadIdx.x; o < e.n && o < base + kChunk32; o += 256) {
+        float pv = to_f(p[o]), mv = m[o], vv = v[o];
+        update32(pv, to_f(g[o]), mv, vv, h);
+        p[o] = from_f<T>(pv); m[o] = mv; v[o] = vv;
+    }
+}
+
+// ---- 8 bits ------------------------------------------------------------------------------------------------------
+// Blocks of 256 elements share two float32 scales, max |m| and max v.  A code k of m stands for sign s (k/127)^2, one of v
+// for s (k/255)^4: steps grow with the value, so m spans 4 and v 9 orders of magnitude below a block's largest.
+//   Rounding: of the two codes around a value the upper one where the value is more than a share u of the way, u from an
+// additive (Weyl) sequence over steps and elements (for v, 1 - u).  Over steps u is spread evenly, so the rounding is
+// unbiased in time; to the nearest code, v would never move: beta2 = 0.999 changes it by 0.1 % a step, codes are at least
+// 1.6 % apart.  v > 0 never becomes 0, which would leave m without its divisor.
+//   The moments and the choice of a code are computed in 64 bits: full rate on this chip, so the codes are the
+// definition's, not a rounding away from it.
+//   A gradient that is not finite leaves its element's moments alone and makes the parameter NaN: a NaN scale would take
+// the other 255 elements along.
+constexpr double kFullM = 127.0 * 127.0, kFullV = 255.0 * 255.0 * 255.0 * 255.0;
+constexpr int kPer8 = 8, kLanes8 = kBlock8 / kPer8, kChunk8 = 256 * kPer8;
+
+// (the float32 nearest to it: the moments that a step starts from are the ones that vsv_adamw_read8 shows)
+__device__ inline float read_m8(int k, double s) { return (float)(s * ((double)(k < 0 ? -k * k : k * k) * (1.0 / kFullM))); }
+__device__ inline float read_v8(unsigned k, double s) { return (float)(s * ((double)(k * k * (k * k)) * (1.0 / kFullV))); }
+
+__device__ inline int code_m8(double x, double inv, double u) {
+    const double y = fmin(fabs(x) * inv, kFullM);
+    double k = (double)(int)__builtin_amdgcn_sqrtf((float)y);
+    if (k * k > y) k -= 1.0;
+    if ((k + 1.0) * (k + 1.0) <= y) k += 1.0;
+    if (y - k * k > u * (2.0 * k + 1.0)) k += 1.0;
+    return x < 0.0 ? -(int)k : (int)k;
+}
+__device__ inline int code_v8(double x, double inv, double u) {
+    const double y = fmin(x * inv, kFullV);
+    double k = (double)(int)__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y));
+    double k2 = k * k, up = (k + 1.0) * (k + 1.0);
+    if (k2 * k2 > y) { up = k2; k -= 1.0; k2 = k * k; }
+    if (up * up <= y) { k2 = up; k += 1.0; up = (k + 1.0) * (k + 1.0); }
+    if (y - k2 * k2 > u * (up * up - k2 * k2)) k += 1.0;
+    return k < 1.0 && x > 0.0 && inv > 0.0 ? 1 : (int)k;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hyper h) {
+    const int ti = tensor_of(tab, blockIdx.x);
+    const vsv_adamw_tensor& e = tab.t[ti];
+    const long o = (long)(blockIdx.x - tab.first[ti]) * kChunk8 + (long)threadIdx.x * kPer8;
+    const long blk = o / kBlock8;
+    if (blk * kBlock8 >= e.n) return;                                     // (a block's 32 lanes leave together)
+    T* p = (T*)e.p; const T* g = (const T*)e.g; int8_t* mc = (int8_t*)e.m; uint8_t* vc = (uint8_t*)e.v;
+    const bool wide = o + kPer8 <= e.n && (((uintptr_t)p | (uintptr_t)g) & 15) == 0 && (((uintptr_t)mc | (uintptr_t)vc) & 7) == 0;
+    const int cnt = o >= e.n ? 0 : e.n - o < kPer8 ? (int)(e.n - o) : kPer8;
+    float pv[kPer8] = {}, gv[kPer8] = {};
+    Pack<int8_t, kPer8> mk = {};
+    Pack<uint8_t, kPer8> vk = {};
+    if (wide) {
+        load_vec<T, kPer8>(p + o, pv); load_vec<T, kPer8>(g + o, gv);
+        mk = *(const Pack<int8_t, kPer8>*)(mc + o);
+        vk = *(const Pack<uint8_t, kPer8>*)(vc + o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPer8; ++j)
+            if (j < cnt) { pv[j] = to_f(p[o + j]); gv[j] = to_f(g[o + j]); mk.v[j] = mc[o + j]; vk.v[j] = vc[o + j]; }
+    }
+    const double ms = e.m_scale[blk], vs = e.v_scale[blk];
+    double m[kPer8], v[kPer8], top_m = 0.0, top_v = 0.0;
+#pragma unroll
+    for (int j = 0; j < kPer8; ++j) {
+        m[j] = read_m8(mk.v[j], ms);
+        v[j] = read_v8(vk.v[j], vs);
+        if (__builtin_isfinite(gv[j])) {
+            const double gd = gv[j];
+            m[j] = m[j] * h.b1d + gd * h.w1d;
+            v[j] = v[j] * h.b2d + gd * gd * h.w2d;
+            pv[j] = pv[j] * h.decay - h.rate * (float)m[j] / (sqrtf((float)v[j]) / h.root + h.eps);
+        } else pv[j] = __builtin_nanf("");
+        top_m = fmax(top_m, fabs(m[j]));
+        top_v = fmax(top_v, v[j]);
+    }
+#pragma unroll
+    for (int w = kLanes8 / 2; w > 0; w >>= 1) {
+        top_m = fmax(top_m, __shfl_xor(top_m, w, kLanes8));
+        top_v = fmax(top_v, __shfl_xor(top_v, w, kLanes8));
+    }
+    const float sm = (float)fmin(top_m, (double)FLT_MAX), sv = (float)fmin(top_v, (double)FLT_MAX);
+    const double im = sm > 0.0f ? kFullM / (double)sm : 0.0, iv = sv > 0.0f ? kFullV / (double)sv : 0.0;
+#pragma unroll
+    for (int j = 0; j < kPer8; ++j) {
+        const unsigned weyl = (unsigned)(o + j) * VSV_ADAMW_WEYL_I + h.dither;
+        const double u = ((double)weyl + 0.5) * (1.0 / 4294967296.0);
+        mk.v[j] = (int8_t)code_m8(m[j], im, u);
+        vk.v[j] = (uint8_t)code_v8(v[j], iv, 1.0 - u);
+    }
+    if (wide) {
+        store_vec<T, kPer8>(p + o, pv);
+        *(Pack<int8_t, kPer8>*)(mc + o) = mk;
+        *(Pack<uint8_t, kPer8>*)(vc + o) = vk;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPer8; ++j)
+            if (j < cnt) { p[o + j] = from_f<T>(pv[j]); mc[o + j] = mk.v[j]; vc[o + j] = vk.v[j]; }
+    }
+    if (threadIdx.x % kLanes8 == 0) { e.m_scale[blk] = sm; e.v_scale[blk] = sv; }
+}
+
+// The values that the codes stand for, in float32: t.p and t.g are the two outputs here.
+__global__ void __launch_bounds__(256) adamw8_read_kernel(const Table tab) {
+    const int ti = tensor_of(tab, blockIdx.x);
+    const vsv_adamw_tensor& e = tab.t[ti];
+    const long base = (long)(blockIdx.x - tab.first[ti]) * kChunk8;
+    const int8_t* mc = (const int8_t*)e.m; const uint8_t* vc = (const uint8_t*)e.v;
+    float *mo = (float*)e.p, *vo = (float*)e.g;
+    for (long o = base + threadIdx.x; o < e.n && o < base + kChunk8; o += 256) {
+        mo[o] = read_m8(mc[o], e.m_scale[o / kBlock8]);
+        vo[o] = read_v8(vc[o], e.v_scale[o / kBlock8]);
+    }
+}
+
+// Launches f(table, workgroups) for every kMaxTensors tensors.
+template <typename F> int over_tables(const vsv_adamw_tensor* t, int n, long chunk, const char* what, F&& f) {
+    for (int at = 0; at < n;) {
+        Table tab;
+        tab.n = 0;
+        long blocks = 0;
+        while (at < n && tab.n < kMaxTensors) {
+            const long b = (t[at].n + chunk - 1) / chunk;
+            if (b > 0x7fffffffL) { set_error("%s: tensor %d is too large", what, at); return -2; }
+            if (blocks + b > 0x7fffffffL) break;
+            if (b > 0) {
+                tab.t[tab.n] = t[at];
+                tab.first[tab.n++] = (unsigned)blocks;
+                blocks += b;
+            }
+            ++at;
+        }
+        if (!blocks) continue;
+        tab.first[tab.n] = (unsigned)blocks;
+        f(tab, (unsigned)blocks);
+        if (int rc = op_launch_check(what)) return rc;
+    }
+    return 0;
+}
+
+int check_tensors(const vsv_adamw_tensor* t, int n, int bits, const char* what) {
+    if (n < 0 || (n > 0 && !t)) { set_error("%s: null table", what); return -1; }
+    if (bits != 8 && bits != 32) { set_error("%s: moments are held in 8 or 32 bits, not %d", what, bits); return -1; }
+    for (int i = 0; i < n; ++i) {
+        if (t[i].n < 0) { set_error("%s: tensor %d has a negative size", what, i); return -1; }
+        if (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (bits == 8 && (!t[i].m_scale || !t[i].v_scale)))) {
+            set_error("%s: tensor %d has a null pointer", what, i); return -1;
+        }
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace vsv
+
+using namespace vsv;
+
+extern "C" int vsv_adamw_multi(const vsv_adamw_tensor* tensors, int n_tensors, int dtype, int bits, double lr, double beta1, double beta2,
+                               double eps, double weight_decay, long step, void* stream) {
+    if (int rc = check_tensors(tensors, n_tensors, bits, "vsv_adamw_multi")) return rc;
+    if (step < 1) { set_error("vsv_adamw_multi: step counts from 1"); return -1; }
+    if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0)) {
+        set_error("vsv_adamw_multi: bad hyper-parameters"); return -1;
+    }
+    Hyper h;
+    h.decay = (float)(1.0 - lr * weight_decay);
+    h.b1 = (float)beta1; h.w1 = (float)(1.0 - beta1); h.b2 = (float)beta2; h.w2 = (float)(1.0 - beta2);
+    h.eps = (float)eps;
+    h.rate = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    h.root = (float)std::sqrt(1.0 - std::pow(beta2, (double)step));
+    h.b1d = beta1; h.w1d = 1.0 - beta1; h.b2d = beta2; h.w2d = 1.0 - beta2;
+    h.dither = (unsigned)step * VSV_ADAMW_WEYL_T;
+    return by_dtype(dtype, "vsv_adamw_multi", [&](auto t) {
+        using T = decltype(t);
+        return over_tables(tensors, n_tensors, bits == 8 ? kChunk8 : kChunk32, "vsv_adamw_multi", [&](const Table& tab, unsigned blocks) {
+            if (bits == 8) hipLaunchKernelGGL(adamw8_kernel<T>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, tab, h);
+            else hipLaunchKernelGGL(adamw32_kernel<T>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, tab, h);
+        });
+    });
+}
+
+extern "C" int vsv_adamw_read8(const vsv_adamw_tensor* tensors, int n_tensors, void* stream) {
+    if (int rc = check_tensors(tensors, n_tensors, 8, "vsv_adamw_read8")) return rc;
+    return over_tables(tensors, n_tensors, kChunk8, "vsv_adamw_read8", [&](const Table& tab, unsigned blocks) {
+        hipLaunchKernelGGL(adamw8_read_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, tab);
+    });
+}

@@ -131,6 +131,39 @@ class VsvLoss(C.Structure):
                 ("weights_dev", C.c_void_p), ("mix", C.c_void_p), ("loss_vec", C.c_void_p), ("ticket", C.c_void_p)]
 
 
+VSV_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}       # VSV_F32, VSV_BF16, VSV_F16
+VSV_CONV_MAX_TAPS = 4
+VSV_SSM_MAX_STATE = 16
+VSV_ADAMW_BLOCK = 256
+
+
+class VsvShortConv(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("K", C.c_int), ("silu", C.c_int), ("B", C.c_long), ("T", C.c_long), ("D", C.c_long),
+                ("x", C.c_void_p), ("x_bs", C.c_long), ("x_ts", C.c_long), ("w", C.c_void_p), ("bias", C.c_void_p),
+                ("state_in", C.c_void_p), ("lengths", C.c_void_p), ("y", C.c_void_p), ("state_out", C.c_void_p)]
+
+
+class VsvShortConvGrads(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("dy_bs", C.c_long), ("dy_ts", C.c_long), ("d_state_out", C.c_void_p)] + \
+               [(n, C.c_void_p) for n in ("dx", "dw", "dbias", "d_state_in")]
+
+
+class VsvSsm(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("N", C.c_int), ("softplus", C.c_int),
+                ("B", C.c_long), ("T", C.c_long), ("D", C.c_long), ("G", C.c_long),
+                ("x", C.c_void_p), ("x_bs", C.c_long), ("x_ts", C.c_long),
+                ("dt", C.c_void_p), ("dt_bs", C.c_long), ("dt_ts", C.c_long),
+                ("gate", C.c_void_p), ("gate_bs", C.c_long), ("gate_ts", C.c_long),
+                ("b", C.c_void_p), ("b_bs", C.c_long), ("b_ts", C.c_long), ("b_gs", C.c_long),
+                ("c", C.c_void_p), ("c_bs", C.c_long), ("c_ts", C.c_long), ("c_gs", C.c_long)] + \
+               [(n, C.c_void_p) for n in ("a", "skip", "dt_bias", "state_in", "lengths", "y", "state_out", "saved")]
+
+
+class VsvSsmGrads(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("dy_bs", C.c_long), ("dy_ts", C.c_long)] + \
+               [(n, C.c_void_p) for n in ("d_state_out", "dx", "ddt", "dgate", "db", "dc", "da", "dskip", "ddt_bias", "d_state_in")]
+
+
 # name -> (restype, argtypes); the full list of symbols include/vsv_hip.h declares
 SIGNATURES = {
     "vsv_abi_version": (C.c_int, []),
@@ -214,6 +247,20 @@ SIGNATURES = {
     "vsv_loss_grad": (C.c_int, [C.POINTER(VsvLoss), C.c_void_p]),
     "vsv_tileb_gemm_launch": (C.c_int, [C.POINTER(VsvTilebGemm), C.c_void_p]),
     "vsv_weight_grads": (C.c_int, [C.POINTER(VsvWgrad), C.c_void_p]),
+    "vsv_short_conv": (C.c_int, [C.POINTER(VsvShortConv), C.c_void_p]),
+    "vsv_short_conv_backward_ws_bytes": (C.c_size_t, [C.POINTER(VsvShortConv)]),
+    "vsv_short_conv_backward": (C.c_int, [C.POINTER(VsvShortConv), C.POINTER(VsvShortConvGrads), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "vsv_short_conv_step": (C.c_int, [C.POINTER(VsvShortConv), C.c_void_p]),
+    "vsv_ssm_saved_floats": (C.c_size_t, [C.POINTER(VsvSsm)]),
+    "vsv_ssm_scan_ws_bytes": (C.c_size_t, [C.POINTER(VsvSsm)]),
+    "vsv_ssm_scan": (C.c_int, [C.POINTER(VsvSsm), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "vsv_ssm_scan_backward_ws_bytes": (C.c_size_t, [C.POINTER(VsvSsm)]),
+    "vsv_ssm_scan_backward": (C.c_int, [C.POINTER(VsvSsm), C.POINTER(VsvSsmGrads), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "vsv_ssm_step": (C.c_int, [C.POINTER(VsvSsm), C.c_void_p]),
+    # (tensors: rows of seven 64-bit words -- p, g, m, v, m_scale, v_scale, n -- as struct vsv_adamw_tensor lays them out)
+    "vsv_adamw_multi": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double,
+                                  C.c_long, C.c_void_p]),
+    "vsv_adamw_read8": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
     "vsv_debug_layout": (C.c_int, [C.POINTER(VsvDims), C.POINTER(C.c_longlong), C.c_int]),
     "vsv_gmm_sample": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_long, C.c_void_p, C.c_void_p,
                                  C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p]),

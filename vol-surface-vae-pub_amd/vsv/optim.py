@@ -1,0 +1,154 @@
+"""AdamW over many tensors in one launch, with moments in 32 bits or in 8 (vsv_adamw_multi).
+
+Beside torch.optim.AdamW, which CVAEMemRand.train_step turns into vsv_adamw_step (float32 parameters whose gradients are one
+flat buffer), this optimizer takes any contiguous float32 / bfloat16 / float16 parameters with gradients of their own, and can
+hold both moments in 8 bits: 2.03 bytes a parameter instead of 8.  It works wherever a torch optimizer does -- schedulers,
+parameter groups, state_dict, and the model classes' train_step(x, optimizer).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import torch
+
+from . import lib as _lib
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW(params, lr, betas, eps, weight_decay, state_bits=32 | 8): decoupled weight decay, bias-corrected moments.
+
+    state_bits=8: per block of 256 elements a float32 scale of each moment; codes are rounded with a dither that is spread
+    evenly over the steps, so small changes of the second moment are not lost.  An element whose gradient is not finite
+    becomes NaN and keeps its moments (with 32 bits its moments follow the gradient).  The state of a parameter is
+    {"step", "exp_avg", "exp_avg_sq"[, "exp_avg_scale", "exp_avg_sq_scale"]}; moments() gives the values in float32.
+
+    The step count is a launch argument, so step() refuses to be captured into a HIP graph."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, not {state_bits!r}")
+        self.state_bits = state_bits
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        try:
+            g = self.param_groups[-1]
+            lr, (b1, b2), eps, wd = float(g["lr"]), g["betas"], g["eps"], g["weight_decay"]
+            if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and wd >= 0.0):
+                raise ValueError(f"AdamW: bad hyper-parameters lr={lr} betas={g['betas']} eps={eps} weight_decay={wd}")
+            for p in g["params"]:
+                _check_param(p)
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _init_state(self, p):
+        st = self.state[p]
+        st["step"] = 0
+        if self.state_bits == 32:
+            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        else:
+            blocks = -(-p.numel() // _lib.VSV_ADAMW_BLOCK)
+            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.int8, device=p.device)
+            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+            st["exp_avg_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lib = _lib.load()
+        work = []                                                          # everything is checked before anything is launched
+        for group in self.param_groups:
+            calls = {}
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                _check_param(p)
+                if g.layout is not torch.strided or g.dtype is not p.dtype or g.device != p.device or g.shape != p.shape:
+                    raise ValueError("AdamW: a gradient needs its parameter's type, device and shape, and no sparse layout")
+                if not p.is_cuda:
+                    raise RuntimeError("AdamW: parameters must be on a GPU; there is no CPU fallback")
+                st = self.state[p]
+                if not st:
+                    st = self._init_state(p)
+                calls.setdefault((p.dtype, p.device, st["step"]), []).append((p, g if g.is_contiguous() else g.contiguous(), st))
+            work += [(group, key, rows) for key, rows in calls.items()]
+        if work and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
+        for group, (dtype, device, step), rows in work:
+            table = _table(rows, self.state_bits)
+            b1, b2 = group["betas"]
+            with torch.cuda.device(device):
+                rc = lib.vsv_adamw_multi(table.ctypes.data, len(rows), _lib.VSV_DTYPES[str(dtype)], self.state_bits, float(group["lr"]),
+                                         float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step + 1,
+                                         C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+            _lib.check(rc, "vsv_adamw_multi")
+            for p, g, st in rows:
+                st["step"] = step + 1
+                torch.autograd.graph.increment_version(p)
+                torch.autograd.graph.increment_version(st["exp_avg"])
+                torch.autograd.graph.increment_version(st["exp_avg_sq"])
+        return loss
+
+    @torch.no_grad()
+    def moments(self):
+        """([exp_avg], [exp_avg_sq]) in float32 of the parameters that have been stepped, in the groups' order: the state's own
+        tensors with 32 bits, the values that the codes stand for with 8."""
+        states = [(p, self.state[p]) for g in self.param_groups for p in g["params"] if self.state.get(p)]
+        if self.state_bits == 32:
+            return [st["exp_avg"] for _, st in states], [st["exp_avg_sq"] for _, st in states]
+        ms = [torch.empty(p.shape, dtype=torch.float32, device=p.device) for p, _ in states]
+        vs = [torch.empty(p.shape, dtype=torch.float32, device=p.device) for p, _ in states]
+        lib = _lib.load()
+        for device in {p.device for p, _ in states}:
+            rows = [(m, v, st) for (p, st), m, v in zip(states, ms, vs) if p.device == device]
+            table = _table(rows, 8)
+            with torch.cuda.device(device):
+                _lib.check(lib.vsv_adamw_read8(table.ctypes.data, len(rows), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)),
+                           "vsv_adamw_read8")
+        return ms, vs
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the moments keep their own types (torch's casts floating state to the parameter's)."""
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, st in state_dict["state"].items():
+            if ("exp_avg_scale" in st) != (self.state_bits == 8):
+                raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
+        super().load_state_dict(state_dict)
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, params):
+            for k, v in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(v):
+                    self.state[p][k] = v.detach().to(device=p.device, copy=True).contiguous()
+                else:
+                    self.state[p][k] = v
+
+
+def _check_param(p):
+    if str(p.dtype) not in _lib.VSV_DTYPES:
+        raise ValueError(f"AdamW: parameters must be float32, bfloat16 or float16, not {p.dtype}")
+    if not p.is_contiguous():
+        raise ValueError("AdamW: parameters must be contiguous")
+
+
+def _table(rows, bits):
+    """struct vsv_adamw_tensor[len(rows)] of (p, g, state) rows, as 64-bit words."""
+    t = np.zeros((len(rows), 7), dtype=np.uint64)
+    t[:, 0] = [p.data_ptr() for p, _, _ in rows]
+    t[:, 1] = [g.data_ptr() for _, g, _ in rows]
+    t[:, 2] = [st["exp_avg"].data_ptr() for _, _, st in rows]
+    t[:, 3] = [st["exp_avg_sq"].data_ptr() for _, _, st in rows]
+    if bits == 8:
+        t[:, 4] = [st["exp_avg_scale"].data_ptr() for _, _, st in rows]
+        t[:, 5] = [st["exp_avg_sq_scale"].data_ptr() for _, _, st in rows]
+    t[:, 6] = [p.numel() for p, _, _ in rows]
+    return t
