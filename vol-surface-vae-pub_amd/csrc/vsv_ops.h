@@ -49,7 +49,7 @@ __device__ inline float softplus_f(float x) {
     p = __builtin_fmaf(p, z, 0x1.99da14p-2f);
     p = __builtin_fmaf(p, z, 0x1.5554e2p-1f);
     p = __builtin_fmaf(p, z, 2.0f);
-    return __builtin_fmaxf(x, 0.0f) + s * p + (x != x ? x : 0.0f);        // (fmax drops a NaN: added back)
+    return __builtin_fmaf(s, p, __builtin_fmaxf(x, 0.0f));                 // (of a NaN, s is one)
 }
 
 template <typename F> int by_dtype(int dtype, const char* what, F&& f) {

@@ -15,7 +15,7 @@ constexpr int kMaxTensors = 60;      // per launch: the argument block stays bel
 constexpr int kBlock8 = VSV_ADAMW_BLOCK;
 
 struct Hyper {
-    float decay, b1, w1, b2, w2, eps, rate, root;
+    float decay, b1, w1, b2, w2, eps, rate, root, inv_root;
     double b1d, w1d, b2d, w2d;
     unsigned dither;
 };
@@ -82,33 +82,55 @@ __global__ void __launch_bounds__(256) adamw32_kernel(const Table tab, const Hyp
 // additive (Weyl) sequence over steps and elements (for v, 1 - u).  Over steps u is spread evenly, so the rounding is
 // unbiased in time; to the nearest code, v would never move: beta2 = 0.999 changes it by 0.1 % a step, codes are at least
 // 1.6 % apart.  v > 0 never becomes 0, which would leave m without its divisor.
-//   The moments and the choice of a code are computed in 64 bits: full rate on this chip, so the codes are the
-// definition's, not a rounding away from it.
+//   The moments are computed in 64 bits (full rate on this chip), and so is the choice of a code wherever float32 could
+// choose another: the codes are the definition's, not a rounding away from it.
 //   A gradient that is not finite leaves its element's moments alone and makes the parameter NaN: a NaN scale would take
 // the other 255 elements along.
 constexpr double kFullM = 127.0 * 127.0, kFullV = 255.0 * 255.0 * 255.0 * 255.0;
 constexpr int kPer8 = 8, kLanes8 = kBlock8 / kPer8, kChunk8 = 256 * kPer8;
 
-// (the float32 nearest to it: the moments that a step starts from are the ones that vsv_adamw_read8 shows)
-__device__ inline float read_m8(int k, double s) { return (float)(s * ((double)(k < 0 ? -k * k : k * k) * (1.0 / kFullM))); }
-__device__ inline float read_v8(unsigned k, double s) { return (float)(s * ((double)(k * k * (k * k)) * (1.0 / kFullV))); }
+// (the float32 nearest to it: the moments that a step starts from are the ones that vsv_adamw_read8 shows; a scale comes
+// divided by the full code's power)
+__device__ inline float read_m8(int k, double s) { const float f = (float)k; return (float)((double)(f * __builtin_fabsf(f)) * s); }
+__device__ inline float read_v8(unsigned k, double s) {
+    const float f = (float)k;
+    const double k2 = (double)(f * f);
+    return (float)(k2 * k2 * s);
+}
 
-__device__ inline int code_m8(double x, double inv, double u) {
+// The codes by the definition, in 64 bits.
+__device__ inline int exact_m8(double x, double inv, double u) {
     const double y = fmin(fabs(x) * inv, kFullM);
     double k = (double)(int)__builtin_amdgcn_sqrtf((float)y);
     if (k * k > y) k -= 1.0;
     if ((k + 1.0) * (k + 1.0) <= y) k += 1.0;
-    if (y - k * k > u * (2.0 * k + 1.0)) k += 1.0;
-    return x < 0.0 ? -(int)k : (int)k;
+    return (int)k + (y - k * k > u * (2.0 * k + 1.0));
 }
-__device__ inline int code_v8(double x, double inv, double u) {
+__device__ inline int exact_v8(double x, double inv, double u) {
     const double y = fmin(x * inv, kFullV);
     double k = (double)(int)__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y));
     double k2 = k * k, up = (k + 1.0) * (k + 1.0);
     if (k2 * k2 > y) { up = k2; k -= 1.0; k2 = k * k; }
     if (up * up <= y) { k2 = up; k += 1.0; up = (k + 1.0) * (k + 1.0); }
-    if (y - k2 * k2 > u * (up * up - k2 * k2)) k += 1.0;
-    return k < 1.0 && x > 0.0 && inv > 0.0 ? 1 : (int)k;
+    return (int)k + (y - k2 * k2 > u * (up * up - k2 * k2));
+}
+// The same in float32, where no more than 2e-5 of a gap is lost: `near` is set where the value lies that close to its
+// threshold, and the 64-bit form decides there.  Next to a code's own value k may come out one off, the share of the gap
+// then next to 1 for next to 0 or the other way round: the code is the same for any u but those next to 0 and 1, which the
+// caller counts as near.
+constexpr float kNear = 1e-4f;
+__device__ inline int code_m8(float x, float inv, float u, bool& near) {
+    const float y = __builtin_fabsf(x) * inv, k = floorf(__builtin_amdgcn_sqrtf(y));
+    const float gap = __builtin_fmaf(2.0f, k, 1.0f), over = __builtin_fmaf(-u, gap, __builtin_fmaf(-k, k, y));
+    near |= __builtin_fabsf(over) < kNear * gap;
+    return (int)k + (over > 0.0f);
+}
+__device__ inline int code_v8(float x, float inv, float u, bool& near) {
+    const float y = x * inv, k = floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(y))), k2 = k * k;
+    const float gap = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(4.0f, k, 6.0f), k, 4.0f), k, 1.0f);
+    const float over = __builtin_fmaf(-u, gap, __builtin_fmaf(-k2, k2, y));
+    near |= __builtin_fabsf(over) < kNear * gap;
+    return (int)k + (over > 0.0f);
 }
 
 template <typename T>
@@ -133,34 +155,60 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hype
         for (int j = 0; j < kPer8; ++j)
             if (j < cnt) { pv[j] = to_f(p[o + j]); gv[j] = to_f(g[o + j]); mk.v[j] = mc[o + j]; vk.v[j] = vc[o + j]; }
     }
-    const double ms = e.m_scale[blk], vs = e.v_scale[blk];
-    double m[kPer8], v[kPer8], top_m = 0.0, top_v = 0.0;
+    const double ms = (double)e.m_scale[blk] * (1.0 / kFullM), vs = (double)e.v_scale[blk] * (1.0 / kFullV);
+    double m[kPer8], v[kPer8];
+    float finite = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPer8; ++j) {
-        m[j] = read_m8(mk.v[j], ms);
-        v[j] = read_v8(vk.v[j], vs);
-        if (__builtin_isfinite(gv[j])) {
-            const double gd = gv[j];
-            m[j] = m[j] * h.b1d + gd * h.w1d;
-            v[j] = v[j] * h.b2d + gd * gd * h.w2d;
-            pv[j] = pv[j] * h.decay - h.rate * (float)m[j] / (sqrtf((float)v[j]) / h.root + h.eps);
-        } else pv[j] = __builtin_nanf("");
-        top_m = fmax(top_m, fabs(m[j]));
-        top_v = fmax(top_v, v[j]);
+        const double gd = gv[j];
+        m[j] = __builtin_fma(gd, h.w1d, (double)read_m8(mk.v[j], ms) * h.b1d);
+        v[j] = __builtin_fma(gd * gd, h.w2d, (double)read_v8(vk.v[j], vs) * h.b2d);
+        finite = __builtin_fmaf(gv[j], 0.0f, finite);
+    }
+    if (finite != 0.0f) {                                                 // some gradient here is not finite
+#pragma unroll
+        for (int j = 0; j < kPer8; ++j)
+            if (!__builtin_isfinite(gv[j])) { m[j] = read_m8(mk.v[j], ms); v[j] = read_v8(vk.v[j], vs); pv[j] = __builtin_nanf(""); }
+    }
+    // (the largest of the values rounded to float32 is the largest value rounded)
+    float m32[kPer8], v32[kPer8], sm = 0.0f, sv = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer8; ++j) {
+        m32[j] = (float)m[j];
+        v32[j] = (float)v[j];
+        sm = __builtin_fmaxf(sm, __builtin_fabsf(m32[j]));
+        sv = __builtin_fmaxf(sv, v32[j]);
+        // the fast root and reciprocal, an ulp each; without an eps subnormal second moments would count, which they lose
+        float den = __builtin_fmaf(__builtin_amdgcn_sqrtf(v32[j]), h.inv_root, h.eps);
+        if (h.eps < 1e-15f) den = __builtin_fmaf((float)sqrt(v[j]), h.inv_root, h.eps);
+        pv[j] = __builtin_fmaf(-h.rate * m32[j], __builtin_amdgcn_rcpf(den), pv[j] * h.decay);
     }
 #pragma unroll
     for (int w = kLanes8 / 2; w > 0; w >>= 1) {
-        top_m = fmax(top_m, __shfl_xor(top_m, w, kLanes8));
-        top_v = fmax(top_v, __shfl_xor(top_v, w, kLanes8));
+        sm = __builtin_fmaxf(sm, __shfl_xor(sm, w, kLanes8));
+        sv = __builtin_fmaxf(sv, __shfl_xor(sv, w, kLanes8));
     }
-    const float sm = (float)fmin(top_m, (double)FLT_MAX), sv = (float)fmin(top_v, (double)FLT_MAX);
+    sm = __builtin_fminf(sm, FLT_MAX);
+    sv = __builtin_fminf(sv, FLT_MAX);
     const double im = sm > 0.0f ? kFullM / (double)sm : 0.0, iv = sv > 0.0f ? kFullV / (double)sv : 0.0;
+    // (float32 holds neither factor where the scale is next to its limits: there, all codes by the definition)
+    const bool plain = (sm > 0.0f && (sm < 1e-30f || sm > 1e30f)) || (sv > 0.0f && (sv < 1e-26f || sv > 1e30f));
+    const float im32 = (float)im, iv32 = (float)iv;
 #pragma unroll
     for (int j = 0; j < kPer8; ++j) {
         const unsigned weyl = (unsigned)(o + j) * VSV_ADAMW_WEYL_I + h.dither;
-        const double u = ((double)weyl + 0.5) * (1.0 / 4294967296.0);
-        mk.v[j] = (int8_t)code_m8(m[j], im, u);
-        vk.v[j] = (uint8_t)code_v8(v[j], iv, 1.0 - u);
+        const float u = (float)weyl * 0x1p-32f;
+        bool near = plain || __builtin_fabsf(u - 0.5f) > 0.5f - kNear;
+        int km = code_m8(m32[j], im32, u, near), kv = code_v8(v32[j], iv32, 1.0f - u, near);
+        if (near) {
+            const double ud = ((double)weyl + 0.5) * 0x1p-32;
+            km = exact_m8(m[j], im, ud);
+            kv = exact_v8(v[j], iv, 1.0 - ud);
+        }
+        const int least = v[j] > 0.0 && sv > 0.0f;
+        kv = kv > least ? kv : least;
+        mk.v[j] = (int8_t)(m32[j] < 0.0f ? -km : km);
+        vk.v[j] = (uint8_t)kv;
     }
     if (wide) {
         store_vec<T, kPer8>(p + o, pv);
@@ -178,13 +226,25 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hype
 __global__ void __launch_bounds__(256) adamw8_read_kernel(const Table tab) {
     const int ti = tensor_of(tab, blockIdx.x);
     const vsv_adamw_tensor& e = tab.t[ti];
-    const long base = (long)(blockIdx.x - tab.first[ti]) * kChunk8;
+    const long o = (long)(blockIdx.x - tab.first[ti]) * kChunk8 + (long)threadIdx.x * kPer8;
+    if (o >= e.n) return;
     const int8_t* mc = (const int8_t*)e.m; const uint8_t* vc = (const uint8_t*)e.v;
     float *mo = (float*)e.p, *vo = (float*)e.g;
-    for (long o = base + threadIdx.x; o < e.n && o < base + kChunk8; o += 256) {
-        mo[o] = read_m8(mc[o], e.m_scale[o / kBlock8]);
-        vo[o] = read_v8(vc[o], e.v_scale[o / kBlock8]);
+    const double ms = (double)e.m_scale[o / kBlock8] * (1.0 / kFullM), vs = (double)e.v_scale[o / kBlock8] * (1.0 / kFullV);
+    if (o + kPer8 <= e.n && (((uintptr_t)mo | (uintptr_t)vo) & 15) == 0 && (((uintptr_t)mc | (uintptr_t)vc) & 7) == 0) {
+        const auto mk = *(const Pack<int8_t, kPer8>*)(mc + o);
+        const auto vk = *(const Pack<uint8_t, kPer8>*)(vc + o);
+#pragma unroll
+        for (int half = 0; half < kPer8; half += 4) {
+            float m[4], v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { m[j] = read_m8(mk.v[half + j], ms); v[j] = read_v8(vk.v[half + j], vs); }
+            store_vec<float, 4>(mo + o + half, m);
+            store_vec<float, 4>(vo + o + half, v);
+        }
+        return;
     }
+    for (int j = 0; j < kPer8 && o + j < e.n; ++j) { mo[o + j] = read_m8(mc[o + j], ms); vo[o + j] = read_v8(vc[o + j], vs); }
 }
 
 // Launches f(table, workgroups) for every kMaxTensors tensors.
@@ -242,6 +302,7 @@ extern "C" int vsv_adamw_multi(const vsv_adamw_tensor* tensors, int n_tensors, i
     h.eps = (float)eps;
     h.rate = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     h.root = (float)std::sqrt(1.0 - std::pow(beta2, (double)step));
+    h.inv_root = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
     h.b1d = beta1; h.w1d = 1.0 - beta1; h.b2d = beta2; h.w2d = 1.0 - beta2;
     h.dither = (unsigned)step * VSV_ADAMW_WEYL_T;
     return by_dtype(dtype, "vsv_adamw_multi", [&](auto t) {

@@ -6,8 +6,6 @@
 namespace vsv {
 namespace {
 
-constexpr int kConvChunk = 32;       // time steps per thread of the convolution
-
 __device__ inline long seq_len(const int* lengths, long b, long T) {
     if (!lengths) return T;
     const long n = lengths[b];
@@ -17,76 +15,102 @@ __device__ inline long seq_len(const int* lengths, long b, long T) {
 // ---- short causal convolution ------------------------------------------------------------------------------------
 // One output from the window, tap by tap and each operation rounded by itself: a prompt and the tokens behind it come out
 // bit for bit the same, whichever kernel computes them, and so does any evaluation that takes the formula at its word -- what
-// is rounded to 16 bits here feeds a recurrent state.  The exponential and the division are the accurate ones; the kernels
-// wait for memory all the same.
+// is rounded to 16 bits here feeds a recurrent state.  The exponential is the accurate one; the quotient 1 / (1 + e) is the
+// reciprocal with one Newton step (a full division costs ten operations more).
 template <int K>
-__device__ inline float conv_out(const float (&w)[K], const float (&x)[K], float bias, int silu) {
+__device__ inline float conv_pre(const float (&w)[K], const float (&x)[K], float bias) {
 #pragma clang fp contract(off)
     float s = w[0] * x[0];
 #pragma unroll
     for (int k = 1; k < K; ++k) s = s + w[k] * x[k];
-    s = s + bias;
-    return silu ? s * (1.0f / (1.0f + expf(-s))) : s;
+    return s + bias;
+}
+__device__ inline float conv_silu(float s) {
+    const float y = __builtin_fminf(1.0f + expf(-s), 3e38f), r = __builtin_amdgcn_rcpf(y);
+    return s * __builtin_fmaf(__builtin_fmaf(-y, r, 1.0f), r, r);
 }
 
 // pre[t,d] = bias[d] + sum_k w[d,k] xs[t-K+1+k, d],  y = silu(pre) or pre; xs is x, continued into state_in before t = 0.
 // One read of x and one write of y (2K flops an element): bound by memory.  A thread owns VEC neighbouring channels and a
-// chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice.
+// chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it works on kRows rows at a
+// time, with the next ones under way.
+constexpr int kRows = 4;
+
+template <typename T, int K, int VEC> struct ConvRows {
+    const T* x;                      // the sequence's row 0, at this thread's channels
+    const float* st;                 // state_in's, or null
+    long ts, D, len;
+    Pack<T, VEC> raw[kRows];
+    __device__ inline ConvRows(const vsv_short_conv_desc& a, long b, long d0)
+        : x((const T*)a.x + b * a.x_bs + d0), st(a.state_in ? a.state_in + b * (K - 1) * a.D + d0 : nullptr), ts(a.x_ts), D(a.D),
+          len(seq_len(a.lengths, b, a.T)) {}
+    __device__ inline void row(long t, float (&out)[VEC]) const {          // xs[t] for any t < len, zeros from there on
+        if (t >= 0 && t < len) { load_vec<T, VEC>(x + t * ts, out); return; }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) out[v] = t < 0 && st ? st[(t + K - 1) * D + v] : 0.0f;
+    }
+    __device__ inline void fetch(long t) {                                 // rows t .. t + kRows - 1; behind the last: the last
+        if (len == 0) return;
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(x + (t + u < len ? t + u : len - 1) * ts);
+    }
+    __device__ inline void take(int u, float (&out)[VEC]) const {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) out[v] = to_f(raw[u].v[v]);
+    }
+};
+
 template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_desc a, long n_chunk, long n_vec) {
+__global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_desc a, long chunk, long n_chunk, long n_vec) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
     if (id >= a.B * n_chunk * n_vec) return;
     const long dv = id % n_vec, bc = id / n_vec, ch = bc % n_chunk, b = bc / n_chunk;
-    const long d0 = dv * VEC, t0 = ch * kConvChunk;
-    const long len = seq_len(a.lengths, b, a.T);
-    const long t1 = t0 + kConvChunk < a.T ? t0 + kConvChunk : a.T;
-    const T* x = (const T*)a.x + b * a.x_bs + d0;
+    const long d0 = dv * VEC, t0 = ch * chunk, t1 = t0 + chunk < a.T ? t0 + chunk : a.T;
     T* y = (T*)a.y + b * a.T * a.D + d0;
-    const float* st = a.state_in ? a.state_in + b * (K - 1) * a.D + d0 : nullptr;
-    float w[K][VEC], bias[VEC], win[K][VEC];
+    ConvRows<T, K, VEC> in(a, b, d0);
+    float w[VEC][K], bias[VEC], xs[K - 1 + kRows][VEC];
+    if (t0 < in.len) in.fetch(t0);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) in.row(t0 - K + 1 + k, xs[k]);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         bias[v] = a.bias ? a.bias[d0 + v] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][v] = a.w[(d0 + v) * K + k];
+        for (int k = 0; k < K; ++k) w[v][k] = a.w[(d0 + v) * K + k];
     }
-    auto row = [&](long t, float (&out)[VEC]) {                           // xs[t], t < len
-        if (t >= 0) { load_vec<T, VEC>(x + t * a.x_ts, out); return; }
+    for (long t = t0; t < t1; t += kRows) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) out[v] = st ? st[(t + K - 1) * a.D + v] : 0.0f;
-    };
+        for (int u = 0; u < kRows; ++u) in.take(u, xs[K - 1 + u]);
+        if (t + kRows < t1 && t + kRows < in.len) in.fetch(t + kRows);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
-        if (t0 - K + 1 + k < len) row(t0 - K + 1 + k, win[k]);
-        else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) win[k][v] = 0.0f;
-        }
-    }
-    for (long t = t0; t < t1; ++t) {
-        float out[VEC];
-        if (t < len) {
-            row(t, win[K - 1]);
+        for (int u = 0; u < kRows; ++u) {
+            if (t + u >= t1) break;
+            float out[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float wv[K], xv[K];
+                float win[K];
 #pragma unroll
-                for (int k = 0; k < K; ++k) { wv[k] = w[k][v]; xv[k] = win[k][v]; }
-                out[v] = conv_out<K>(wv, xv, bias[v], a.silu);
-#pragma unroll
-                for (int k = 0; k < K - 1; ++k) win[k][v] = win[k + 1][v];
+                for (int k = 0; k < K; ++k) win[k] = xs[u + k][v];
+                out[v] = conv_pre<K>(w[v], win, bias[v]);
             }
-        } else {
+            if (a.silu) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) out[v] = 0.0f;
+                for (int v = 0; v < VEC; ++v) out[v] = conv_silu(out[v]);
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) out[v] = t + u < in.len ? out[v] : 0.0f;
+            store_vec<T, VEC>(y + (t + u) * a.D, out);
         }
-        store_vec<T, VEC>(y + t * a.D, out);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) xs[k][v] = xs[k + kRows][v];
     }
     if (a.state_out && ch == 0) {
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
             float r[VEC];
-            row(len - (K - 1) + j, r);
+            in.row(in.len - (K - 1) + j, r);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) a.state_out[(b * (K - 1) + j) * a.D + d0 + v] = r[v];
         }
@@ -95,100 +119,99 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
 
 // ds = dy act'(pre) (pre computed again from x), dx[t] = sum_k w[k] ds[t+K-1-k], dw[k] = sum_t ds[t] xs[t-K+1+k],
 // dbias = sum_t ds.  The same chunks; a chunk reads K-1 rows beyond each end, its sums over time go to `part`
-// (chunk, K + 1, D) and are joined in a fixed order by sum_rows_kernel.
+// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.
 template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_conv_desc a, const vsv_short_conv_grads g, long n_chunk,
+__global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_conv_desc a, const vsv_short_conv_grads g, long chunk, long n_chunk,
                                                              long n_vec, float* __restrict__ part) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
     if (id >= a.B * n_chunk * n_vec) return;
     const long dv = id % n_vec, bc = id / n_vec, ch = bc % n_chunk, b = bc / n_chunk;
-    const long d0 = dv * VEC, t0 = ch * kConvChunk;
-    const long len = seq_len(a.lengths, b, a.T);
-    const long t1 = t0 + kConvChunk < a.T ? t0 + kConvChunk : a.T;
-    const T* x = (const T*)a.x + b * a.x_bs + d0;
+    const long d0 = dv * VEC, t0 = ch * chunk, t1 = t0 + chunk < a.T ? t0 + chunk : a.T;
     const T* dy = (const T*)g.dy + b * g.dy_bs + d0;
     T* dx = (T*)g.dx + b * a.T * a.D + d0;
-    const float* st = a.state_in ? a.state_in + b * (K - 1) * a.D + d0 : nullptr;
     const float* dso = g.d_state_out ? g.d_state_out + b * (K - 1) * a.D + d0 : nullptr;
-    float w[K][VEC], bias[VEC], win[K][VEC], dsw[K][VEC], dw[K][VEC], db[VEC];
+    ConvRows<T, K, VEC> in(a, b, d0);
+    Pack<T, VEC> dyr[kRows];
+    auto fetch = [&](long t) {
+        in.fetch(t);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) dyr[u] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (t + u < in.len ? t + u : in.len - 1) * g.dy_ts);
+    };
+    float w[K][VEC], bias[VEC], xs[K - 1 + kRows][VEC], ds[K - 1 + kRows][VEC], dw[K][VEC], db[VEC];
+    if (t0 < in.len) fetch(t0);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+        in.row(t0 - K + 1 + k, xs[k]);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) ds[k][v] = 0.0f;
+    }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         bias[v] = a.bias ? a.bias[d0 + v] : 0.0f;
         db[v] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) { w[k][v] = a.w[(d0 + v) * K + k]; dsw[k][v] = 0.0f; dw[k][v] = 0.0f; }
+        for (int k = 0; k < K; ++k) { w[k][v] = a.w[(d0 + v) * K + k]; dw[k][v] = 0.0f; }
     }
-    auto row = [&](long t, float (&out)[VEC]) {
-        if (t >= 0) { load_vec<T, VEC>(x + t * a.x_ts, out); return; }
+    const long lo = ch == 0 ? -(K - 1) : t0, end = t1 + K - 1;            // (chunk 0 also returns the state's gradient)
+    for (long t = t0; t < end; t += kRows) {
+        float dyv[kRows][VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) out[v] = st ? st[(t + K - 1) * a.D + v] : 0.0f;
-    };
+        for (int u = 0; u < kRows; ++u) {
+            in.take(u, xs[K - 1 + u]);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
-        if (t0 - K + 1 + k < len) row(t0 - K + 1 + k, win[k]);
-        else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) win[k][v] = 0.0f;
+            for (int v = 0; v < VEC; ++v) dyv[u][v] = to_f(dyr[u].v[v]);
         }
-    }
-    const long lo = ch == 0 ? -(K - 1) : t0;                              // (chunk 0 also returns the state's gradient)
-    for (long t = t0; t < t1 + K - 1; ++t) {
+        if (t + kRows < end && t + kRows < in.len) fetch(t + kRows);
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) dsw[k][v] = dsw[k + 1][v];      // dsw[K-1-k] = ds[t-k]
-        if (t < len) {
-            float dyv[VEC];
-            row(t, win[K - 1]);
-            load_vec<T, VEC>(dy + t * g.dy_ts, dyv);
+        for (int u = 0; u < kRows; ++u) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float ds = dyv[v];
+                float d = dyv[u][v];
                 if (a.silu) {
                     float s = bias[v];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], win[k][v], s);
+                    for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], xs[u + k][v], s);
                     const float sg = sigmoid_f(s);
-                    ds *= sg * (1.0f + s * (1.0f - sg));
+                    d *= sg * __builtin_fmaf(s, 1.0f - sg, 1.0f);
                 }
-                dsw[K - 1][v] = ds;
-                if (t < t1) {
-                    db[v] += ds;
+                if (t + u >= in.len) d = 0.0f;
+                ds[K - 1 + u][v] = d;
+                if (t + u < t1 && t + u < in.len) {
+                    db[v] += d;
 #pragma unroll
-                    for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(ds, win[k][v], dw[k][v]);
+                    for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d, xs[u + k][v], dw[k][v]);
                 }
-#pragma unroll
-                for (int k = 0; k < K - 1; ++k) win[k][v] = win[k + 1][v];
             }
-        } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) dsw[K - 1][v] = 0.0f;
         }
-        const long to = t - (K - 1);
-        if (to < lo) continue;
-        float o[VEC];
-        const long j = to - (len - (K - 1));                              // the row of state_out that xs[to] is, if any
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float s = 0.0f;
+        for (int u = 0; u < kRows; ++u) {
+            const long to = t + u - (K - 1);                              // dx of this row: ds[to + K-1-k] is ds[u + K-1-k] here
+            if (to < lo || to >= t1) continue;
+            float o[VEC];
+            const long j = to - (in.len - (K - 1));                       // the row of state_out that xs[to] is, if any
 #pragma unroll
-            for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], dsw[K - 1 - k][v], s);
-            if (dso && j >= 0 && j < K - 1) s += dso[j * a.D + v];
-            o[v] = s;
+            for (int v = 0; v < VEC; ++v) {
+                float s = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], ds[u + K - 1 - k][v], s);
+                if (dso && j >= 0 && j < K - 1) s += dso[j * a.D + v];
+                o[v] = s;
+            }
+            if (to >= 0) store_vec<T, VEC>(dx + to * a.D, o);
+            else if (g.d_state_in) {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) g.d_state_in[(b * (K - 1) + to + K - 1) * a.D + d0 + v] = o[v];
+            }
         }
-        if (to >= 0) store_vec<T, VEC>(dx + to * a.D, o);
-        else if (g.d_state_in) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) g.d_state_in[(b * (K - 1) + to + K - 1) * a.D + d0 + v] = o[v];
-        }
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) { xs[k][v] = xs[k + kRows][v]; ds[k][v] = ds[k + kRows][v]; }
     }
     float* p = part + (b * n_chunk + ch) * (K + 1) * a.D + d0;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) p[k * a.D + v] = dw[k][v];
-        p[(long)K * a.D + v] = db[v];
-    }
+    for (int k = 0; k < K; ++k) store_vec<float, VEC>(p + k * a.D, dw[k]);
+    store_vec<float, VEC>(p + (long)K * a.D, db);
 }
 
 // out_j = sum over rows of part (rows, M); element m = k * D + d goes to dw[d * K + k] or, k == K, to dbias[d].
@@ -198,8 +221,10 @@ __global__ void __launch_bounds__(256) sum_conv_parts_kernel(const float* __rest
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long M = (K + 1) * D, m = (long)blockIdx.x * 64 + lane;
     float s = 0.0f;
-    if (m < M)
+    if (m < M) {
+#pragma unroll 8
         for (long r = wave; r < rows; r += 4) s += part[r * M + m];
+    }
     red[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && m < M) {
@@ -224,7 +249,8 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
     float wv[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) wv[k] = w[d * K + k];
-    y[b * D + d] = from_f<T>(conv_out<K>(wv, win, bias ? bias[d] : 0.0f, silu));
+    const float s = conv_pre<K>(wv, win, bias ? bias[d] : 0.0f);
+    y[b * D + d] = from_f<T>(silu ? conv_silu(s) : s);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) state[(b * (K - 1) + k) * D + d] = win[k + 1];
 }
@@ -234,23 +260,17 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
 // The decay belongs to (channel, state), so there is no matrix form: per state and step one exponential and four float32
 // operations, 24 cycles of a SIMD per 64 channels, against 8 bytes of traffic per channel and step in 16 bits.  Bound by
 // the vector units.
-//   A lane owns a channel and its N states (padded to R) in registers, a wave 64 channels of one group.  b_t and c_t are
-// the same for the whole wave: they are read through the scalar cache into scalar registers and cost no vector work and
-// no shared memory.  x, dt and gate of the next kTile steps are loaded while the present ones are computed; the
-// activations are taken for a tile at a time.
+//   A lane owns a channel and its N states (padded to R) in registers, a wave 64 channels of one group, which share b_t and
+// c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are computed; the activations are
+// taken for a tile at a time.
 //   A wave runs along time alone, so where sequences and channels make fewer waves than the chip has SIMDs the time axis is
 // split (scan_plan).  A first pass gives every segment's state from zero and its sum of delta; the state in front of a
 // segment then follows from exp(a sum delta), one step per earlier segment, at the start of the second pass.
 constexpr int kTile = 8;             // steps per tile; training keeps the state before every tile
 
-typedef const __attribute__((address_space(4))) uint32_t* ScalarU;
-
 struct ScanPlan {
     long seg;                        // steps per segment, a multiple of kTile
     int S;                           // segments
-    // b and c as the kernels read them: in place, or as float32 rows of R states that pack_bc_kernel wrote
-    const void *b, *c;
-    long b_bs, b_ts, b_gs, c_bs, c_ts, c_gs;
 };
 
 struct ScanPos {
@@ -286,35 +306,68 @@ __device__ inline ScanPos scan_pos(const vsv_ssm_desc& a, const ScanPlan& pl, un
     return p;
 }
 
-// n states of b_t or c_t, uniform over the wave, as the words that scalar loads bring.  BF: pairs of bfloat16 in place, else
-// float32.  Scalar loads return out of order, so a wait is for all of them: every step waits for its own rows first, then
-// asks for the next step's, and computes while these are on their way (scheduling barriers keep that order).
-template <int R, bool BF> struct ScalarRow {
-    uint32_t w[BF ? R / 2 : R];
-    __device__ inline void load(uintptr_t p) {
-        const ScalarU u = (ScalarU)p;
-#pragma unroll
-        for (int j = 0; j < (BF ? R / 2 : R); ++j) w[j] = u[j];
-    }
-    __device__ inline float at(int n) const {
-        if (!BF) return __builtin_bit_cast(float, w[n]);
-        return __builtin_bit_cast(float, n & 1 ? w[n / 2] & 0xffff0000u : w[n / 2] << 16);
-    }
-};
-__device__ inline void order() { __builtin_amdgcn_sched_barrier(0); }
 // An empty statement that a value passes through: what is computed from it stays behind it, in its step.  (Without it the
 // steps of a tile are computed side by side, and their states do not fit the registers.)
 __device__ inline void pin(float& v) { asm volatile("" : "+v"(v)); }
-__device__ inline void scalar_wait() { __builtin_amdgcn_s_waitcnt(0xc07f); order(); }      // lgkmcnt(0)
+__device__ inline void order() { __builtin_amdgcn_sched_barrier(0); }
 
-// kTile rows from `row` on (those behind the first `left` repeat the last) of one channel per lane; `row` is uniform
-template <typename T>
-__device__ inline void load_tile(const T* row, long ts, unsigned lane, int left, T (&out)[kTile]) {
-#pragma unroll
-    for (int i = 0; i < kTile; ++i) {
-        out[i] = row[lane];
-        if (i + 1 < left) row += ts;
+// b and c of a tile: eight lanes to a step, four of them b's states and four c's, R / 4 each.  They are loaded a tile ahead,
+// whatever their strides, and laid down in the wave's own shared memory as float32, zeros behind the N states; a step then
+// reads its rows as broadcasts.  (Read through the scalar cache, with the next step's rows under way during the present
+// step, a wave alone on its SIMD took 1080 cycles a step: the scalar loads miss to L2, and only the latest can be waited for.)
+template <typename T, int R> struct BcTile {
+    static constexpr int V = R / 4;
+    const T* at;                     // this lane's first state in the tile's first row of its own
+    long ts;
+    int row, n0, to;
+    bool on;
+    T raw[V];
+    __device__ inline BcTile(const vsv_ssm_desc& a, const ScanPos& p, long t, bool use_b, bool use_c) {
+        const int l = threadIdx.x, c = (l >> 2) & 1;
+        row = l >> 3;
+        n0 = (l & 3) * V;
+        to = row * 2 * R + c * R + n0;
+        on = c ? use_c : use_b;
+        ts = c ? a.c_ts : a.b_ts;
+        at = (const T*)(c ? a.c : a.b) + p.b * (c ? a.c_bs : a.b_bs) + p.g * (c ? a.c_gs : a.b_gs) + (t + row) * ts + n0;
     }
+    __device__ inline void fetch(int N, int left) {                       // rows behind the first `left` repeat the last
+        if (!on) return;
+        const T* q = at;
+        if (left < kTile && row >= left) q -= (row - left + 1) * ts;
+#pragma unroll
+        for (int k = 0; k < V; ++k) raw[k] = n0 + k < N ? q[k] : from_f<T>(0.0f);
+    }
+    __device__ inline void move(int tiles) { at += (long)tiles * kTile * ts; }
+    __device__ inline void lay(float* lds) const {
+        float v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = to_f(raw[k]);
+        if (on) store_vec<float, V>(lds + to, v);
+    }
+};
+// H states of a row, the same for every lane
+template <int H> __device__ inline void bc_row(const float* lds, float (&v)[H]) {
+#pragma unroll
+    for (int k = 0; k < H / 4; ++k) {
+        float q[4];
+        load_vec<float, 4>(lds + 4 * k, q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * k + j] = q[j];
+    }
+}
+
+// One channel per lane of kTile rows from `row` on, `step` bytes apart (rows behind the first `left` repeat the last):
+// buffer loads, whose per-row address is one scalar offset.
+template <typename T> __device__ inline T buffer_get(__amdgpu_buffer_rsrc_t r, unsigned voff, int soff) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, soff, 0));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, (int)voff, soff, 0));
+}
+template <typename T>
+__device__ inline void load_tile(const T* row, int step, unsigned lane, int left, T (&out)[kTile]) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, -1, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) out[i] = buffer_get<T>(r, lane * (unsigned)sizeof(T), (i < left ? i : left - 1) * step);
 }
 
 // The time steps and inputs of a tile; steps at t1 and beyond get delta = x = 0, which leaves every state as it is.
@@ -341,11 +394,26 @@ template <typename T> __device__ inline void tile_values(const T (&r)[kTile], in
             if (i >= left) v[i] = 0.0f;
     }
 }
-template <typename T> __device__ inline void tile_store(T* base, long D, const ScanPos& p, long t, int left, const float (&v)[kTile]) {
-    if (!p.live) return;
+// (a dead lane's offset lies behind the buffer's end, where stores are dropped)
+template <typename T> __device__ inline void tile_store(T* row, long D, const ScanPos& p, int left, const float (&v)[kTile]) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(row, 0, 0x7fffffff, 0x00020000);
+    const int voff = p.live ? (int)(p.lane * (unsigned)sizeof(T)) : (int)0xfffffff0;
+    const int step = (int)(D * (long)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < kTile; ++i)
-        if (i < left) (base + (t + i) * D)[p.lane] = from_f<T>(v[i]);
+    for (int i = 0; i < kTile; ++i) {
+        if (left < kTile && i >= left) break;
+        const T o = from_f<T>(v[i]);
+        if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, o), r, voff, i * step, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, o), r, voff, i * step, 0);
+    }
+}
+
+// decay_n = exp(delta a_n), all of them before the first is used: an exponential's result is late
+template <int R> __device__ inline void decays(float de, const float* A2, float (&e)[R]) {
+#pragma unroll
+    for (int n = 0; n < R; ++n) e[n] = de * A2[n];
+#pragma unroll
+    for (int n = 0; n < R; ++n) e[n] = exp2_fast(e[n]);
 }
 
 // State sets in memory: (R/4, D, 4), so that a wave moves 1 KiB at a time.
@@ -387,48 +455,46 @@ __device__ inline void fold_segments(const float* E, const float* sd, long D, lo
 }
 
 // First pass of a split scan: a segment's last state from zero, and its sum of delta.
-template <typename T, int R, bool BF>
+template <typename T, int R>
 __global__ void __launch_bounds__(64) ssm_ends_kernel(const vsv_ssm_desc a, const ScanPlan pl, float* __restrict__ E, float* __restrict__ sd) {
-    constexpr long kEl = BF ? 2 : 4;
+    __shared__ alignas(16) float lds[2][kTile * 2 * R];
     const ScanPos p = scan_pos(a, pl, blockIdx.x, 0);
     const long D = a.D, d = p.base + p.lane;
     float A2[R], h[R] = {}, sum = 0.0f;
     load_decay<R>(a, d, A2);
     const float dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     const T *x = (const T*)a.x + p.b * a.x_bs + p.base + p.t0 * a.x_ts, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + p.t0 * a.dt_ts;
-    uintptr_t pb = (uintptr_t)pl.b + (p.b * pl.b_bs + p.g * pl.b_gs + p.t0 * pl.b_ts) * kEl;
-    ScalarRow<R, BF> b;
+    BcTile<T, R> bc(a, p, p.t0, true, false);
     T xr[kTile], dr[kTile];
-    if (p.t0 < p.t1) {
-        b.load(pb);
-        load_tile(x, a.x_ts, p.lane, tile_left(p, p.t0), xr);
-        load_tile(dt, a.dt_ts, p.lane, tile_left(p, p.t0), dr);
-    }
-    for (long t = p.t0; t < p.t1; t += kTile) {
+    auto fetch = [&](int left) {
+        bc.fetch(a.N, left);
+        load_tile(x, (int)(a.x_ts * (long)sizeof(T)), p.lane, left, xr);
+        load_tile(dt, (int)(a.dt_ts * (long)sizeof(T)), p.lane, left, dr);
+    };
+    if (p.t0 < p.t1) fetch(tile_left(p, p.t0));
+    int buf = 0;
+    for (long t = p.t0; t < p.t1; t += kTile, buf ^= 1) {
         const int left = tile_left(p, t);
-        const bool more = t + kTile < p.t1;
         float xv[kTile], raw[kTile], de[kTile];
+        bc.lay(lds[buf]);
         tile_values(xr, left, xv);
         tile_steps(dr, dtb, a.softplus, left, raw, de);
-        if (more) {
-            x += kTile * a.x_ts; dt += kTile * a.dt_ts;
-            load_tile(x, a.x_ts, p.lane, tile_left(p, t + kTile), xr);
-            load_tile(dt, a.dt_ts, p.lane, tile_left(p, t + kTile), dr);
+        if (t + kTile < p.t1) {
+            x += kTile * a.x_ts; dt += kTile * a.dt_ts; bc.move(1);
+            fetch(tile_left(p, t + kTile));
         }
         order();
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            ScalarRow<R, BF> nb;
-            scalar_wait();
-            if (i + 1 < left || more) pb += pl.b_ts * kEl;
-            nb.load(pb);
-            order();
+            float b[R], e[R];
+            bc_row<R>(lds[buf] + i * 2 * R, b);
             const float dx = de[i] * xv[i];
+            decays<R>(de[i], A2, e);
             sum += de[i];
-#pragma unroll
-            for (int n = 0; n < R; ++n) h[n] = __builtin_fmaf(exp2_fast(de[i] * A2[n]), h[n], dx * b.at(n));
             order();
-            b = nb;
+#pragma unroll
+            for (int n = 0; n < R; ++n) h[n] = __builtin_fmaf(e[n], h[n], dx * b[n]);
+            order();
         }
     }
     if (!p.live) return;
@@ -436,37 +502,37 @@ __global__ void __launch_bounds__(64) ssm_ends_kernel(const vsv_ssm_desc a, cons
     sd[(p.b * pl.S + p.s) * D + d] = sum;
 }
 
-template <typename T, int R, bool BF>
+template <typename T, int R>
 __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, const ScanPlan pl, const float* __restrict__ E,
                                                       const float* __restrict__ sd) {
-    constexpr long kEl = BF ? 2 : 4;
+    __shared__ alignas(16) float lds[2][kTile * 2 * R];
     const ScanPos p = scan_pos(a, pl, blockIdx.x, 0);
     const long D = a.D, d = p.base + p.lane;
     const int N = a.N;
     T* y = (T*)a.y + p.b * a.T * D + p.base;
+    const T *x = (const T*)a.x + p.b * a.x_bs + p.base + p.t0 * a.x_ts, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + p.t0 * a.dt_ts;
+    const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base + p.t0 * a.gate_ts : nullptr;
+    BcTile<T, R> bc(a, p, p.t0, true, true);
+    T xr[kTile], dr[kTile], gr[kTile];
+    auto fetch = [&](int left) {
+        bc.fetch(N, left);
+        load_tile(x, (int)(a.x_ts * (long)sizeof(T)), p.lane, left, xr);
+        load_tile(dt, (int)(a.dt_ts * (long)sizeof(T)), p.lane, left, dr);
+        if (gate) load_tile(gate, (int)(a.gate_ts * (long)sizeof(T)), p.lane, left, gr);
+    };
+    if (p.t0 < p.t1) fetch(tile_left(p, p.t0));
     float A2[R], h[R];
     load_decay<R>(a, d, A2);
 #pragma unroll
     for (int n = 0; n < R; ++n) h[n] = n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n] : 0.0f;
     fold_segments<R>(E, sd, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
     const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
-    const T *x = (const T*)a.x + p.b * a.x_bs + p.base + p.t0 * a.x_ts, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + p.t0 * a.dt_ts;
-    const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base + p.t0 * a.gate_ts : nullptr;
-    uintptr_t pb = (uintptr_t)pl.b + (p.b * pl.b_bs + p.g * pl.b_gs + p.t0 * pl.b_ts) * kEl;
-    uintptr_t pc = (uintptr_t)pl.c + (p.b * pl.c_bs + p.g * pl.c_gs + p.t0 * pl.c_ts) * kEl;
     float* saved = a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D : nullptr;
-    ScalarRow<R, BF> b, c;
-    T xr[kTile], dr[kTile], gr[kTile];
-    auto fetch = [&](int left) {
-        load_tile(x, a.x_ts, p.lane, left, xr);
-        load_tile(dt, a.dt_ts, p.lane, left, dr);
-        if (gate) load_tile(gate, a.gate_ts, p.lane, left, gr);
-    };
-    if (p.t0 < p.t1) { b.load(pb); c.load(pc); fetch(tile_left(p, p.t0)); }
-    for (long t = p.t0; t < p.t1; t += kTile) {
+    int buf = 0;
+    for (long t = p.t0; t < p.t1; t += kTile, buf ^= 1) {
         const int left = tile_left(p, t);
-        const bool more = t + kTile < p.t1;
         float xv[kTile], raw[kTile], de[kTile], gv[kTile], yv[kTile];
+        bc.lay(lds[buf]);
         tile_values(xr, left, xv);
         tile_steps(dr, dtb, a.softplus, left, raw, de);
         if (gate) {
@@ -474,8 +540,8 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
 #pragma unroll
             for (int i = 0; i < kTile; ++i) gv[i] *= sigmoid_f(gv[i]);
         }
-        if (more) {
-            x += kTile * a.x_ts; dt += kTile * a.dt_ts; gate += gate ? kTile * a.gate_ts : 0;
+        if (t + kTile < p.t1) {
+            x += kTile * a.x_ts; dt += kTile * a.dt_ts; gate += gate ? kTile * a.gate_ts : 0; bc.move(1);
             fetch(tile_left(p, t + kTile));
         }
         if (saved) {
@@ -485,27 +551,25 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
         order();
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            ScalarRow<R, BF> nb, nc;
-            scalar_wait();
-            if (i + 1 < left || more) { pb += pl.b_ts * kEl; pc += pl.c_ts * kEl; }
-            nb.load(pb); nc.load(pc);
-            order();
+            float b[R], c[R], e[R], acc[2] = {skip * xv[i], 0.0f};
+            bc_row<R>(lds[buf] + i * 2 * R, b);
+            bc_row<R>(lds[buf] + i * 2 * R + R, c);
             const float dx = de[i] * xv[i];
-            float acc = skip * xv[i];
+            decays<R>(de[i], A2, e);
+            order();
 #pragma unroll
             for (int n = 0; n < R; ++n) {
-                h[n] = __builtin_fmaf(exp2_fast(de[i] * A2[n]), h[n], dx * b.at(n));
-                acc = __builtin_fmaf(c.at(n), h[n], acc);
+                h[n] = __builtin_fmaf(e[n], h[n], dx * b[n]);
+                acc[n & 1] = __builtin_fmaf(c[n], h[n], acc[n & 1]);
             }
-            yv[i] = acc;
+            yv[i] = acc[0] + acc[1];
             order();
-            b = nb; c = nc;
         }
         if (gate) {
 #pragma unroll
             for (int i = 0; i < kTile; ++i) yv[i] *= gv[i];
         }
-        tile_store(y, D, p, t, left, yv);
+        tile_store(y + t * D, D, p, left, yv);
     }
     if (!p.live) return;
     for (long t = p.t0 > p.t1 ? p.t0 : p.t1; t < p.tz; ++t) (y + t * D)[p.lane] = from_f<T>(0.0f);
@@ -517,10 +581,10 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
 
 // Backwards: g = dy silu(gate), q_t = c_t g_t + exp(delta_{t+1} a) q_{t+1} is the gradient of h_t.
 // First pass of a split one: the gradient of the state in front of a segment where none comes in from behind it.
-template <typename T, int R, bool BF>
+template <typename T, int R>
 __global__ void __launch_bounds__(64) ssm_bwd_ends_kernel(const vsv_ssm_desc a, const vsv_ssm_grads gr, const ScanPlan pl, float* __restrict__ E,
                                                           float* __restrict__ sd) {
-    constexpr long kEl = BF ? 2 : 4;
+    __shared__ alignas(16) float lds[2][kTile * 2 * R];
     const ScanPos p = scan_pos(a, pl, blockIdx.x, 1);
     const long D = a.D, d = p.base + p.lane;
     float A2[R], q[R] = {}, sum = 0.0f;
@@ -529,19 +593,20 @@ __global__ void __launch_bounds__(64) ssm_bwd_ends_kernel(const vsv_ssm_desc a, 
     const long tl = p.t0 + (p.t1 - 1 - p.t0) / kTile * kTile;              // the last tile
     const T *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + tl * a.dt_ts, *dy = (const T*)gr.dy + p.b * gr.dy_bs + p.base + tl * gr.dy_ts;
     const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base + tl * a.gate_ts : nullptr;
-    uintptr_t pc = (uintptr_t)pl.c + (p.b * pl.c_bs + p.g * pl.c_gs + (p.t1 - 1) * pl.c_ts) * kEl;
-    ScalarRow<R, BF> c;
+    BcTile<T, R> bc(a, p, tl, false, true);
     T dr[kTile], gtr[kTile], yr[kTile];
     auto fetch = [&](int left) {
-        load_tile(dt, a.dt_ts, p.lane, left, dr);
-        load_tile(dy, gr.dy_ts, p.lane, left, yr);
-        if (gate) load_tile(gate, a.gate_ts, p.lane, left, gtr);
+        bc.fetch(a.N, left);
+        load_tile(dt, (int)(a.dt_ts * (long)sizeof(T)), p.lane, left, dr);
+        load_tile(dy, (int)(gr.dy_ts * (long)sizeof(T)), p.lane, left, yr);
+        if (gate) load_tile(gate, (int)(a.gate_ts * (long)sizeof(T)), p.lane, left, gtr);
     };
-    if (p.t0 < p.t1) { c.load(pc); fetch(tile_left(p, tl)); }
-    for (long t = tl; t >= p.t0 && p.t0 < p.t1; t -= kTile) {
+    if (p.t0 < p.t1) fetch(tile_left(p, tl));
+    int buf = 0;
+    for (long t = tl; t >= p.t0 && p.t0 < p.t1; t -= kTile, buf ^= 1) {
         const int left = tile_left(p, t);
-        const bool more = t > p.t0;
         float raw[kTile], de[kTile], g[kTile];
+        bc.lay(lds[buf]);
         tile_steps(dr, dtb, a.softplus, left, raw, de);
         tile_values(yr, left, g);
         if (gate) {
@@ -550,23 +615,21 @@ __global__ void __launch_bounds__(64) ssm_bwd_ends_kernel(const vsv_ssm_desc a, 
 #pragma unroll
             for (int i = 0; i < kTile; ++i) g[i] *= gv[i] * sigmoid_f(gv[i]);
         }
-        if (more) {
-            dt -= kTile * a.dt_ts; dy -= kTile * gr.dy_ts; gate -= gate ? kTile * a.gate_ts : 0;
+        if (t > p.t0) {
+            dt -= kTile * a.dt_ts; dy -= kTile * gr.dy_ts; gate -= gate ? kTile * a.gate_ts : 0; bc.move(-1);
             fetch(kTile);
         }
         order();
 #pragma unroll
         for (int i = kTile - 1; i >= 0; --i) {
-            ScalarRow<R, BF> nc;
-            scalar_wait();
-            if (i < left && (i > 0 || more)) pc -= pl.c_ts * kEl;
-            nc.load(pc);
-            order();
+            float c[R], e[R];
+            bc_row<R>(lds[buf] + i * 2 * R + R, c);
+            decays<R>(de[i], A2, e);
             sum += de[i];
-#pragma unroll
-            for (int n = 0; n < R; ++n) q[n] = exp2_fast(de[i] * A2[n]) * __builtin_fmaf(c.at(n), g[i], q[n]);
             order();
-            if (i < left) c = nc;
+#pragma unroll
+            for (int n = 0; n < R; ++n) q[n] = e[n] * __builtin_fmaf(c[n], g[i], q[n]);
+            order();
         }
     }
     if (!p.live) return;
@@ -611,12 +674,12 @@ template <int NV> __device__ inline float wave_sums(float (&v)[NV]) {
 
 // A tile at a time from the state saved in front of it: its states are computed again into registers, then q runs through
 // them in reverse, four states at a time so that they fit.  The gradients of b and c are sums over channels: over the
-// wave's 64 here, over the channel blocks in sum_bc_kernel; those of a, skip and dt_bias sums over time: here, and over
-// sequences and segments in sum_params_kernel.  All in a fixed order.
-template <typename T, int R, bool BF>
+// wave's 64 here, over the channel blocks in ssm_sums_kernel; those of a, skip and dt_bias sums over time: here, and over
+// sequences and segments there too.  All in a fixed order.
+template <typename T, int R>
 __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, const vsv_ssm_grads gr, const ScanPlan pl, const float* __restrict__ E,
                                                         const float* __restrict__ sd, float* __restrict__ part_bc, float* __restrict__ part_p) {
-    constexpr long kEl = BF ? 2 : 4;
+    __shared__ alignas(16) float lds[2][kTile * 2 * R];
     constexpr int H = 4;
     const ScanPos p = scan_pos(a, pl, blockIdx.x, 0);
     const long D = a.D, d = p.base + p.lane;
@@ -628,8 +691,6 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
     const float* saved = a.saved + (p.b * ((a.T + kTile - 1) / kTile) + tl / kTile) * R * D;
     const long row = p.b * a.T * D + p.base;
     T *dx_o = (T*)gr.dx + row, *ddt_o = (T*)gr.ddt + row, *dg_o = gate ? (T*)gr.dgate + row : nullptr;
-    uintptr_t pb = (uintptr_t)pl.b + (p.b * pl.b_bs + p.g * pl.b_gs + tl * pl.b_ts) * kEl;
-    uintptr_t pc = (uintptr_t)pl.c + (p.b * pl.c_bs + p.g * pl.c_gs + tl * pl.c_ts) * kEl;
     const long Dg = D / a.G, blk = (p.base - p.g * Dg) / 64;
     float* bc = part_bc + (((blk * a.B + p.b) * a.T) * a.G + p.g) * (2 * R);
     const long bc_ts = a.G * 2 * R;
@@ -644,17 +705,21 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
     }
     const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     float dskip = 0.0f, ddtb = 0.0f;
+    BcTile<T, R> bct(a, p, tl, true, true);
     T xr[kTile], dr[kTile], gtr[kTile], yr[kTile];
     auto fetch = [&](int left) {
-        load_tile(x, a.x_ts, p.lane, left, xr);
-        load_tile(dt, a.dt_ts, p.lane, left, dr);
-        load_tile(dy, gr.dy_ts, p.lane, left, yr);
-        if (gate) load_tile(gate, a.gate_ts, p.lane, left, gtr);
+        bct.fetch(N, left);
+        load_tile(x, (int)(a.x_ts * (long)sizeof(T)), p.lane, left, xr);
+        load_tile(dt, (int)(a.dt_ts * (long)sizeof(T)), p.lane, left, dr);
+        load_tile(dy, (int)(gr.dy_ts * (long)sizeof(T)), p.lane, left, yr);
+        if (gate) load_tile(gate, (int)(a.gate_ts * (long)sizeof(T)), p.lane, left, gtr);
     };
     if (p.t0 < p.t1) fetch(tile_left(p, tl));
-    for (long t = tl; t >= p.t0 && p.t0 < p.t1; t -= kTile) {
+    int buf = 0;
+    for (long t = tl; t >= p.t0 && p.t0 < p.t1; t -= kTile, buf ^= 1) {
         const int left = tile_left(p, t);
         float h0[R], xv[kTile], raw[kTile], de[kTile], g[kTile], dsl[kTile];
+        bct.lay(lds[buf]);
         load_states<R>(saved, D, d, h0);
         tile_values(xr, left, xv);
         tile_steps(dr, dtb, a.softplus, left, raw, de);
@@ -675,59 +740,49 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
         }
         if (t > p.t0) {
             x -= kTile * a.x_ts; dt -= kTile * a.dt_ts; dy -= kTile * gr.dy_ts; gate -= gate ? kTile * a.gate_ts : 0;
-            saved -= R * D;
+            saved -= R * D; bct.move(-1);
             fetch(kTile);
         }
         float qb[kTile] = {}, dde[kTile] = {}, yv[kTile] = {};
 #pragma unroll
         for (int n0 = 0; n0 < R; n0 += H) {
             float hs[kTile + 1][H];
-            ScalarRow<H, BF> b, c, nb, nc;
-            b.load(pb + n0 * kEl);
 #pragma unroll
             for (int n = 0; n < H; ++n) hs[0][n] = h0[n0 + n];
-            uintptr_t rb = pb + n0 * kEl;
             order();
 #pragma unroll
             for (int i = 0; i < kTile; ++i) {
-                scalar_wait();
-                if (i + 1 < left) rb += pl.b_ts * kEl;
-                if (i + 1 < kTile) nb.load(rb);
-                else c.load(pc + (n0 + (left - 1) * pl.c_ts) * kEl);       // (b stays: the reverse starts at the same row)
-                order();
-                float dei = de[i];
+                float b[H], e[H], dei = de[i];
+                bc_row<H>(lds[buf] + i * 2 * R + n0, b);
                 pin(dei);
                 const float dx = dei * xv[i];
+                decays<H>(dei, A2 + n0, e);
+                order();
 #pragma unroll
                 for (int n = 0; n < H; ++n) {
-                    hs[i + 1][n] = __builtin_fmaf(exp2_fast(dei * A2[n0 + n]), hs[i][n], dx * b.at(n));
+                    hs[i + 1][n] = __builtin_fmaf(e[n], hs[i][n], dx * b[n]);
                     pin(hs[i + 1][n]);
                 }
                 order();
-                if (i + 1 < kTile) b = nb;
             }
-            uintptr_t rc = pc + (n0 + (left - 1) * pl.c_ts) * kEl;
 #pragma unroll
             for (int i = kTile - 1; i >= 0; --i) {
-                float v[2 * H];
-                scalar_wait();
-                if (i > 0) {
-                    if (i < left) { rb -= pl.b_ts * kEl; rc -= pl.c_ts * kEl; }
-                    nb.load(rb); nc.load(rc);
-                }
-                order();
-                float dei = de[i];
+                float b[H], c[H], e[H], v[2 * H], dei = de[i];
+                bc_row<H>(lds[buf] + i * 2 * R + n0, b);
+                bc_row<H>(lds[buf] + i * 2 * R + R + n0, c);
                 pin(dei);
                 const float dx = dei * xv[i];
+                decays<H>(dei, A2 + n0, e);
+                order();
 #pragma unroll
                 for (int n = 0; n < H; ++n) {
                     float& qn = q[n0 + n];
-                    qn = __builtin_fmaf(c.at(n), g[i], qn);
-                    yv[i] = __builtin_fmaf(c.at(n), hs[i + 1][n], yv[i]);
-                    qb[i] = __builtin_fmaf(b.at(n), qn, qb[i]);
+                    qn = __builtin_fmaf(c[n], g[i], qn);
+                    yv[i] = __builtin_fmaf(c[n], hs[i + 1][n], yv[i]);
+                    qb[i] = __builtin_fmaf(b[n], qn, qb[i]);
                     v[n] = qn * dx;
                     v[H + n] = g[i] * hs[i + 1][n];
-                    qn *= exp2_fast(dei * A2[n0 + n]);
+                    qn *= e[n];
                     const float w = qn * hs[i][n];
                     dde[i] = __builtin_fmaf(A2[n0 + n], w, dde[i]);
                     dA[n0 + n] = __builtin_fmaf(dei, w, dA[n0 + n]);
@@ -737,14 +792,12 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
                 const float sum = wave_sums<2 * H>(v);
                 constexpr int kEach = 64 / (2 * H);
                 if (i < left && threadIdx.x % kEach == 0) {
-                    const int j = threadIdx.x / kEach;                      // b's four states, then c's
+                    const int j = threadIdx.x / kEach;                      // b's H states, then c's
                     bc[(t + i) * bc_ts + n0 + (j < H ? j : j - H + R)] = sum;
                 }
                 order();
-                b = nb; c = nc;
             }
         }
-        pb -= kTile * pl.b_ts * kEl; pc -= kTile * pl.c_ts * kEl;
         float dxv[kTile], ddv[kTile];
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
@@ -754,12 +807,12 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
             ddtb += ddv[i];
             dxv[i] = __builtin_fmaf(qb[i], de[i], g[i] * skip);
         }
-        tile_store(dx_o, D, p, t, left, dxv);
-        tile_store(ddt_o, D, p, t, left, ddv);
+        tile_store(dx_o + t * D, D, p, left, dxv);
+        tile_store(ddt_o + t * D, D, p, left, ddv);
         if (gate) {
 #pragma unroll
             for (int i = 0; i < kTile; ++i) yv[i] = dsl[i] * __builtin_fmaf(skip, xv[i], yv[i]);
-            tile_store(dg_o, D, p, t, left, yv);
+            tile_store(dg_o + t * D, D, p, left, yv);
         }
     }
     for (long t = p.t0 > p.t1 ? p.t0 : p.t1; t < p.tz; ++t) {
@@ -782,45 +835,31 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
             if (n < N) gr.d_state_in[(p.b * D + d) * N + n] = q[n];
 }
 
-// b and c (any strides, N states) as float32 rows (B, T, G, 2, R), padded with zeros: what the scalar loads need where the
-// tensors themselves are not whole, aligned words.
+// The last sums of the backward pass, in a fixed order.  Workgroups below bc_blocks: db, dc from the channel blocks' shares
+// (blocks, B T G, 2 R), rounded once; the others: da, dskip, d_dt_bias from the sequences' and segments' (rows, R + 2, D).
 template <typename T>
-__global__ void __launch_bounds__(256) pack_bc_kernel(const vsv_ssm_desc a, int R, float* __restrict__ out) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.B * a.T * a.G * 2 * R) return;
-    const int j = (int)(id % (2 * R)), n = j < R ? j : j - R;
-    const long r = id / (2 * R), g = r % a.G, bt = r / a.G, t = bt % a.T, b = bt / a.T;
-    float v = 0.0f;
-    if (n < a.N)
-        v = to_f(j < R ? ((const T*)a.b)[b * a.b_bs + t * a.b_ts + g * a.b_gs + n] : ((const T*)a.c)[b * a.c_bs + t * a.c_ts + g * a.c_gs + n]);
-    out[id] = v;
-}
-
-// db, dc: the channel blocks' shares (blocks, B T G, 2 R) joined in order and rounded once
-template <typename T>
-__global__ void __launch_bounds__(256) sum_bc_kernel(const float* __restrict__ part, long blocks, long rows, int R, int N,
-                                                     T* __restrict__ db, T* __restrict__ dc) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x, M = rows * 2 * R;
-    if (id >= M) return;
-    const long r = id / (2 * R);
-    const int j = (int)(id - r * 2 * R), n = j < R ? j : j - R;
-    if (n >= N) return;
-    float s = 0.0f;
-#pragma unroll 8
-    for (long k = 0; k < blocks; ++k) s += part[k * M + id];
-    (j < R ? db : dc)[r * N + n] = from_f<T>(s);
-}
-
-// da, dskip, d_dt_bias: the sequences' and segments' shares (rows, R + 2, D) joined in order
-__global__ void __launch_bounds__(256) sum_params_kernel(const float* __restrict__ part, long rows, long D, int R, int N,
-                                                         float* __restrict__ da, float* __restrict__ dskip, float* __restrict__ ddtb) {
+__global__ void __launch_bounds__(256) ssm_sums_kernel(const float* __restrict__ part, long blocks, long bc_rows, unsigned bc_blocks, int R, int N,
+                                                       T* __restrict__ db, T* __restrict__ dc, const float* __restrict__ part_p, long rows,
+                                                       long D, float* __restrict__ da, float* __restrict__ dskip, float* __restrict__ ddtb) {
     __shared__ float red[4][64];
+    if (blockIdx.x < bc_blocks) {
+        const long id = (long)blockIdx.x * 256 + threadIdx.x, M = bc_rows * 2 * R;
+        if (id >= M) return;
+        const long r = id / (2 * R);
+        const int j = (int)(id - r * 2 * R), n = j < R ? j : j - R;
+        if (n >= N) return;
+        float s = 0.0f;
+#pragma unroll 8
+        for (long k = 0; k < blocks; ++k) s += part[k * M + id];
+        (j < R ? db : dc)[r * N + n] = from_f<T>(s);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long M = (R + 2) * D, m = (long)blockIdx.x * 64 + lane;
+    const long M = (R + 2) * D, m = (long)(blockIdx.x - bc_blocks) * 64 + lane;
     float s = 0.0f;
     if (m < M) {
 #pragma unroll 8
-        for (long r = wave; r < rows; r += 4) s += part[r * M + m];
+        for (long r = wave; r < rows; r += 4) s += part_p[r * M + m];
     }
     red[wave][lane] = s;
     __syncthreads();
@@ -896,7 +935,15 @@ bool conv_wide(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, size
     return ok;
 }
 
-long conv_chunks(const vsv_short_conv_desc* a) { return a->T > 0 ? (a->T + kConvChunk - 1) / kConvChunk : 1; }
+// Time steps per thread: the longer, the less is read twice and the fewer sums are left over, as long as there are two waves
+// for every SIMD (131072 threads).
+long conv_chunk(const vsv_short_conv_desc* a) {
+    const long vecs = a->D / (a->D % 8 == 0 ? 8 : 1), rows = a->B * vecs;
+    long chunk = 16;
+    while (chunk < 256 && rows * ((a->T + 2 * chunk - 1) / (2 * chunk)) >= 131072) chunk *= 2;
+    return chunk;
+}
+long conv_chunks(const vsv_short_conv_desc* a) { const long c = conv_chunk(a); return a->T > 0 ? (a->T + c - 1) / c : 1; }
 
 template <typename F> int by_taps(int K, F&& f) {
     switch (K) {
@@ -913,6 +960,10 @@ int check_ssm(const vsv_ssm_desc* a, const char* what) {
     if (a->B < 0 || a->T < 0 || a->D < 1) { set_error("%s: bad sizes (B %ld, T %ld, D %ld)", what, a->B, a->T, a->D); return -1; }
     if (a->G < 1 || a->D % a->G) { set_error("%s: %ld channels do not divide into %ld groups", what, a->D, a->G); return -1; }
     if (a->dtype < VSV_F32 || a->dtype > VSV_F16) { set_error("%s: dtype must be VSV_F32, VSV_BF16 or VSV_F16", what); return -1; }
+    const long most = 0x7fffffffL / (4 * 8);                             // (the scan addresses eight rows with 32 bits)
+    if (a->D > most || a->x_ts > most || a->dt_ts > most || a->gate_ts > most || a->x_ts < 0 || a->dt_ts < 0 || a->gate_ts < 0) {
+        set_error("%s: a time stride of more than %ld elements, or a negative one", what, most); return -2;
+    }
     if (!a->a || (a->B > 0 && a->T > 0 && (!a->x || !a->dt || !a->b || !a->c || !a->y))) { set_error("%s: null pointer", what); return -1; }
     return 0;
 }
@@ -929,17 +980,17 @@ template <typename F> int by_states(int N, F&& f) {
 
 long ssm_blocks(const vsv_ssm_desc* a) { return (a->D / a->G + 63) / 64; }
 
-// The scan's split of time.  A second pass over a segment costs 1.8 times one pass over it, so a split pays below about
-// half a wave per SIMD (1024 of them): from there on as many segments as make two waves per SIMD, none shorter than two
+// The scan's split of time.  A split costs a second pass (1.8 times the work) and a launch, so it pays below half a wave per
+// SIMD (1024 of them) and from kSplitFrom steps on: then as many segments as make two waves per SIMD, none shorter than two
 // tiles, at most kMaxSegments (the start of a segment walks over those in front of it).
-constexpr long kMaxSegments = 64;
+constexpr long kMaxSegments = 64, kSplitFrom = 128, kSplitWaves = 2048;
 
 ScanPlan scan_plan(const vsv_ssm_desc* a) {
     ScanPlan pl = {};
     const long waves = a->B * a->G * ssm_blocks(a), tiles = (a->T + kTile - 1) / kTile;
     long S = 1;
-    if (waves > 0 && waves < 512 && tiles >= 4) {
-        S = (2048 + waves - 1) / waves;
+    if (waves > 0 && waves < 512 && a->T >= kSplitFrom) {
+        S = (kSplitWaves + waves - 1) / waves;
         if (S > tiles / 2) S = tiles / 2;
         if (S > kMaxSegments) S = kMaxSegments;
     }
@@ -949,50 +1000,10 @@ ScanPlan scan_plan(const vsv_ssm_desc* a) {
     return pl;
 }
 
-// Whether scalar loads can read b and c in place: whole rows of R states in float32, or in bfloat16 on 4 bytes.
-bool bc_in_place(const vsv_ssm_desc* a) {
-    if (a->N != padded_states(a->N)) return false;
-    if (a->dtype == VSV_F32) return true;
-    return a->dtype == VSV_BF16 && aligned(a->b, 4) && aligned(a->c, 4) &&
-           ((a->b_bs | a->b_ts | a->b_gs | a->c_bs | a->c_ts | a->c_gs) & 1) == 0;
-}
-
-size_t bc_floats(const vsv_ssm_desc* a) { return bc_in_place(a) ? 0 : (size_t)a->B * a->T * a->G * 2 * padded_states(a->N); }
 size_t ends_floats(const vsv_ssm_desc* a, const ScanPlan& pl) {
     return pl.S > 1 ? (size_t)a->B * pl.S * (padded_states(a->N) + 1) * a->D : 0;
 }
 size_t round4(size_t n) { return (n + 3) & ~(size_t)3; }
-
-// Points the plan at b and c, packing them into `out` first where they cannot be read in place.
-template <typename T> int place_bc(const vsv_ssm_desc* a, ScanPlan& pl, float* out, void* stream, const char* what) {
-    if (bc_in_place(a)) {
-        pl.b = a->b; pl.b_bs = a->b_bs; pl.b_ts = a->b_ts; pl.b_gs = a->b_gs;
-        pl.c = a->c; pl.c_bs = a->c_bs; pl.c_ts = a->c_ts; pl.c_gs = a->c_gs;
-        return 0;
-    }
-    const int R = padded_states(a->N);
-    pl.b = out; pl.c = out + R;
-    pl.b_gs = pl.c_gs = 2 * R;
-    pl.b_ts = pl.c_ts = a->G * 2 * R;
-    pl.b_bs = pl.c_bs = a->T * a->G * 2 * R;
-    const long blocks = ((long)bc_floats(a) + 255) / 256;
-    if (blocks == 0) return 0;
-    if (blocks > kMaxBlocks) { set_error("%s: too many elements for one call", what); return -2; }
-    hipLaunchKernelGGL(pack_bc_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, R, out);
-    return op_launch_check("pack_bc_kernel");
-}
-
-// f(T, R, whether b and c are pairs of bfloat16 in place)
-template <typename F> int by_scan(const vsv_ssm_desc* a, const char* what, F&& f) {
-    return by_dtype(a->dtype, what, [&](auto t) {
-        return by_states(a->N, [&](auto r) {
-            if constexpr (std::is_same<decltype(t), __bf16>::value) {
-                if (bc_in_place(a)) return f(t, r, std::true_type{});
-            }
-            return f(t, r, std::false_type{});
-        });
-    });
-}
 
 }  // namespace
 }  // namespace vsv
@@ -1009,8 +1020,8 @@ extern "C" int vsv_short_conv(const vsv_short_conv_desc* a, void* stream) {
             const bool wide = conv_wide(a, nullptr, sizeof(T), V);
             const long nc = conv_chunks(a), nv = wide ? a->D / V : a->D, blocks = (a->B * nc * nv + 255) / 256;
             if (blocks > kMaxBlocks) { set_error("vsv_short_conv: too many elements for one call"); return -2; }
-            if (wide) hipLaunchKernelGGL((short_conv_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, nc, nv);
-            else hipLaunchKernelGGL((short_conv_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, nc, nv);
+            if (wide) hipLaunchKernelGGL((short_conv_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a), nc, nv);
+            else hipLaunchKernelGGL((short_conv_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a), nc, nv);
             return op_launch_check("short_conv_kernel");
         });
     });
@@ -1030,12 +1041,12 @@ extern "C" int vsv_short_conv_backward(const vsv_short_conv_desc* a, const vsv_s
         const int rc = by_dtype(a->dtype, "vsv_short_conv_backward", [&](auto t) {
             using T = decltype(t);
             return by_taps(a->K, [&](auto k) {
-                constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
+                constexpr int K = decltype(k)::value, V = 4;              // (eight channels a thread would need all its registers)
                 const bool wide = conv_wide(a, g, sizeof(T), V);
                 const long nv = wide ? a->D / V : a->D, blocks = (a->B * nc * nv + 255) / 256;
                 if (blocks > kMaxBlocks) { set_error("vsv_short_conv_backward: too many elements for one call"); return -2; }
-                if (wide) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, nc, nv, (float*)ws);
-                else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, nc, nv, (float*)ws);
+                if (wide) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a), nc, nv, (float*)ws);
+                else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a), nc, nv, (float*)ws);
                 return op_launch_check("short_conv_bwd_kernel");
             });
         });
@@ -1068,7 +1079,7 @@ extern "C" size_t vsv_ssm_saved_floats(const vsv_ssm_desc* a) {
 
 extern "C" size_t vsv_ssm_scan_ws_bytes(const vsv_ssm_desc* a) {
     if (check_ssm(a, "vsv_ssm_scan_ws_bytes")) return 0;
-    return (round4(bc_floats(a)) + ends_floats(a, scan_plan(a))) * sizeof(float);
+    return ends_floats(a, scan_plan(a)) * sizeof(float);
 }
 
 extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, void* stream) {
@@ -1077,22 +1088,20 @@ extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, vo
     const size_t need = vsv_ssm_scan_ws_bytes(a);
     if (ws_bytes < need || (need && !aligned(ws, 16)) || (need && !ws)) { set_error("vsv_ssm_scan: workspace too small or not on 16 bytes"); return -1; }
     if (a->saved && !aligned(a->saved, 16)) { set_error("vsv_ssm_scan: saved must be on 16 bytes"); return -1; }
-    ScanPlan pl = scan_plan(a);
+    const ScanPlan pl = scan_plan(a);
     const long waves = a->B * a->G * ssm_blocks(a);
-    if (waves * pl.S > kMaxBlocks) { set_error("vsv_ssm_scan: too many sequences and channels for one call"); return -2; }
-    float *bc = (float*)ws, *E = bc + round4(bc_floats(a)), *sd = E + (size_t)a->B * pl.S * padded_states(a->N) * a->D;
-    return by_scan(a, "vsv_ssm_scan", [&](auto t, auto r, auto bf) {
+    if (waves > kMaxBlocks / pl.S) { set_error("vsv_ssm_scan: too many sequences and channels for one call"); return -2; }
+    float *E = (float*)ws, *sd = E + (size_t)a->B * pl.S * padded_states(a->N) * a->D;
+    return by_dtype(a->dtype, "vsv_ssm_scan", [&](auto t) { return by_states(a->N, [&](auto r) {
         using T = decltype(t);
         constexpr int R = decltype(r)::value;
-        constexpr bool BF = decltype(bf)::value;
-        if (int rc = place_bc<T>(a, pl, bc, stream, "vsv_ssm_scan")) return rc;
         if (pl.S > 1) {
-            hipLaunchKernelGGL((ssm_ends_kernel<T, R, BF>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+            hipLaunchKernelGGL((ssm_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
             if (int rc = op_launch_check("ssm_ends_kernel")) return rc;
         }
-        hipLaunchKernelGGL((ssm_scan_kernel<T, R, BF>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+        hipLaunchKernelGGL((ssm_scan_kernel<T, R>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
         return op_launch_check("ssm_scan_kernel");
-    });
+    }); });
 }
 
 namespace {
@@ -1102,7 +1111,7 @@ size_t part_bc_floats(const vsv_ssm_desc* a) { return (size_t)ssm_blocks(a) * a-
 extern "C" size_t vsv_ssm_scan_backward_ws_bytes(const vsv_ssm_desc* a) {
     if (check_ssm(a, "vsv_ssm_scan_backward_ws_bytes")) return 0;
     const ScanPlan pl = scan_plan(a);
-    return (round4(bc_floats(a)) + round4(ends_floats(a, pl)) + round4(part_bc_floats(a)) +
+    return (round4(ends_floats(a, pl)) + round4(part_bc_floats(a)) +
             (size_t)a->B * pl.S * (padded_states(a->N) + 2) * a->D) * sizeof(float);
 }
 
@@ -1111,36 +1120,38 @@ extern "C" int vsv_ssm_scan_backward(const vsv_ssm_desc* a, const vsv_ssm_grads*
     if (!g || (a->B > 0 && a->T > 0 && (!a->saved || !g->dy || !g->dx || !g->ddt || !g->db || !g->dc || (a->gate && !g->dgate)))) {
         set_error("vsv_ssm_scan_backward: null pointer"); return -1;
     }
+    if (g->dy_ts < 0 || g->dy_ts > 0x7fffffffL / (4 * 8)) { set_error("vsv_ssm_scan_backward: bad time stride of dy"); return -2; }
     if (ws_bytes < vsv_ssm_scan_backward_ws_bytes(a) || (a->B > 0 && (!ws || !aligned(ws, 16)))) {
         set_error("vsv_ssm_scan_backward: workspace too small or not on 16 bytes"); return -1;
     }
     if (a->saved && !aligned(a->saved, 16)) { set_error("vsv_ssm_scan_backward: saved must be on 16 bytes"); return -1; }
-    ScanPlan pl = scan_plan(a);
+    const ScanPlan pl = scan_plan(a);
     const int R0 = padded_states(a->N);
     const long nb = ssm_blocks(a), waves = a->B * a->G * nb, rows = a->B * a->T * a->G;
-    if (waves * pl.S > kMaxBlocks || (rows * 2 * R0 + 255) / 256 > kMaxBlocks) { set_error("vsv_ssm_scan_backward: too many elements for one call"); return -2; }
-    float *bc = (float*)ws, *E = bc + round4(bc_floats(a)), *sd = E + (size_t)a->B * pl.S * R0 * a->D;
+    if (waves > kMaxBlocks / pl.S) { set_error("vsv_ssm_scan_backward: too many elements for one call"); return -2; }
+    float *E = (float*)ws, *sd = E + (size_t)a->B * pl.S * R0 * a->D;
     float *pbc = E + round4(ends_floats(a, pl)), *pp = pbc + round4(part_bc_floats(a));
     if (a->B > 0) {
-        const int rc = by_scan(a, "vsv_ssm_scan_backward", [&](auto t, auto r, auto bf) {
+        const int rc = by_dtype(a->dtype, "vsv_ssm_scan_backward", [&](auto t) { return by_states(a->N, [&](auto r) {
             using T = decltype(t);
             constexpr int R = decltype(r)::value;
-            constexpr bool BF = decltype(bf)::value;
-            if (int rc = place_bc<T>(a, pl, bc, stream, "vsv_ssm_scan_backward")) return rc;
-            if (pl.S > 1) {
-                hipLaunchKernelGGL((ssm_bwd_ends_kernel<T, R, BF>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd);
+                if (pl.S > 1) {
+                hipLaunchKernelGGL((ssm_bwd_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd);
                 if (int rc = op_launch_check("ssm_bwd_ends_kernel")) return rc;
             }
-            hipLaunchKernelGGL((ssm_bwd_kernel<T, R, BF>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd, pbc, pp);
-            if (int rc = op_launch_check("ssm_bwd_kernel")) return rc;
-            if (rows == 0) return 0;
-            hipLaunchKernelGGL(sum_bc_kernel<T>, dim3((unsigned)((rows * 2 * R + 255) / 256)), dim3(256), 0, (hipStream_t)stream, pbc, nb, rows, R, a->N, (T*)g->db, (T*)g->dc);
-            return op_launch_check("sum_bc_kernel");
-        });
+            hipLaunchKernelGGL((ssm_bwd_kernel<T, R>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd, pbc, pp);
+            return op_launch_check("ssm_bwd_kernel");
+        }); });
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(sum_params_kernel, dim3((unsigned)(((R0 + 2) * a->D + 63) / 64)), dim3(256), 0, (hipStream_t)stream, pp, a->B * pl.S, a->D, R0, a->N, g->da, g->dskip, g->ddt_bias);
-    return op_launch_check("sum_params_kernel");
+    const long bc_blocks = (rows * 2 * R0 + 255) / 256, blocks = bc_blocks + ((R0 + 2) * a->D + 63) / 64;
+    if (blocks > kMaxBlocks) { set_error("vsv_ssm_scan_backward: too many elements for one call"); return -2; }
+    return by_dtype(a->dtype, "vsv_ssm_scan_backward", [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(ssm_sums_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, pbc, nb, rows, (unsigned)bc_blocks, R0, a->N,
+                           (T*)g->db, (T*)g->dc, pp, a->B * pl.S, a->D, g->da, g->dskip, g->ddt_bias);
+        return op_launch_check("ssm_sums_kernel");
+    });
 }
 
 extern "C" int vsv_ssm_step(const vsv_ssm_desc* a, void* stream) {

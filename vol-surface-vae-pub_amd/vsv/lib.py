@@ -131,7 +131,6 @@ class VsvLoss(C.Structure):
                 ("weights_dev", C.c_void_p), ("mix", C.c_void_p), ("loss_vec", C.c_void_p), ("ticket", C.c_void_p)]
 
 
-VSV_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}       # VSV_F32, VSV_BF16, VSV_F16
 VSV_CONV_MAX_TAPS = 4
 VSV_SSM_MAX_STATE = 16
 VSV_ADAMW_BLOCK = 256

@@ -7,12 +7,12 @@ parameter groups, state_dict, and the model classes' train_step(x, optimizer).
 """
 from __future__ import annotations
 
-import ctypes as C
+import array
 
-import numpy as np
 import torch
 
 from . import lib as _lib
+from .ssm import _TYPES, _call, _touched
 
 
 class AdamW(torch.optim.Optimizer):
@@ -64,57 +64,51 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib = _lib.load()
-        work = []                                                          # everything is checked before anything is launched
-        for group in self.param_groups:
-            calls = {}
+        state, calls = self.state, []
+        for group in self.param_groups:                                    # everything is checked before anything is launched
+            rows = {}
             for p in group["params"]:
                 g = p.grad
                 if g is None:
                     continue
-                _check_param(p)
-                if g.layout is not torch.strided or g.dtype is not p.dtype or g.device != p.device or g.shape != p.shape:
+                if p.dtype not in _TYPES or not p.is_contiguous():
+                    _check_param(p)
+                if g.layout is not torch.strided or g.dtype is not p.dtype or g.get_device() != p.get_device() or g.shape != p.shape:
                     raise ValueError("AdamW: a gradient needs its parameter's type, device and shape, and no sparse layout")
                 if not p.is_cuda:
                     raise RuntimeError("AdamW: parameters must be on a GPU; there is no CPU fallback")
-                st = self.state[p]
-                if not st:
-                    st = self._init_state(p)
-                calls.setdefault((p.dtype, p.device, st["step"]), []).append((p, g if g.is_contiguous() else g.contiguous(), st))
-            work += [(group, key, rows) for key, rows in calls.items()]
-        if work and torch.cuda.is_current_stream_capturing():
+                st = state[p] or self._init_state(p)
+                rows.setdefault((p.dtype, p.get_device(), st["step"]), []).append((p, g if g.is_contiguous() else g.contiguous(), st))
+            calls += [(group, *key, rows[key]) for key in rows]
+        if calls and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
-        for group, (dtype, device, step), rows in work:
+        for group, dtype, at, step, rows in calls:
             table = _table(rows, self.state_bits)
             b1, b2 = group["betas"]
-            with torch.cuda.device(device):
-                rc = lib.vsv_adamw_multi(table.ctypes.data, len(rows), _lib.VSV_DTYPES[str(dtype)], self.state_bits, float(group["lr"]),
-                                         float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step + 1,
-                                         C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
-            _lib.check(rc, "vsv_adamw_multi")
-            for p, g, st in rows:
+            _call("vsv_adamw_multi", at, table.buffer_info()[0], len(rows), _TYPES[dtype], self.state_bits, float(group["lr"]),
+                  float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step + 1)
+            written = []
+            for p, _, st in rows:
                 st["step"] = step + 1
-                torch.autograd.graph.increment_version(p)
-                torch.autograd.graph.increment_version(st["exp_avg"])
-                torch.autograd.graph.increment_version(st["exp_avg_sq"])
+                written += (p, st["exp_avg"], st["exp_avg_sq"])
+            _touched(written)
         return loss
 
     @torch.no_grad()
     def moments(self):
         """([exp_avg], [exp_avg_sq]) in float32 of the parameters that have been stepped, in the groups' order: the state's own
         tensors with 32 bits, the values that the codes stand for with 8."""
-        states = [(p, self.state[p]) for g in self.param_groups for p in g["params"] if self.state.get(p)]
+        states = [st for st in (self.state.get(p) for g in self.param_groups for p in g["params"]) if st]
         if self.state_bits == 32:
-            return [st["exp_avg"] for _, st in states], [st["exp_avg_sq"] for _, st in states]
-        ms = [torch.empty(p.shape, dtype=torch.float32, device=p.device) for p, _ in states]
-        vs = [torch.empty(p.shape, dtype=torch.float32, device=p.device) for p, _ in states]
-        lib = _lib.load()
-        for device in {p.device for p, _ in states}:
-            rows = [(m, v, st) for (p, st), m, v in zip(states, ms, vs) if p.device == device]
-            table = _table(rows, 8)
-            with torch.cuda.device(device):
-                _lib.check(lib.vsv_adamw_read8(table.ctypes.data, len(rows), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)),
-                           "vsv_adamw_read8")
+            return [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
+        ms = [torch.empty_like(st["exp_avg"], dtype=torch.float32) for st in states]
+        vs = [torch.empty_like(m) for m in ms]
+        rows = {}
+        for m, v, st in zip(ms, vs, states):
+            rows.setdefault(m.get_device(), []).append((m, v, st))
+        for at, part in rows.items():
+            table = _table(part, 8)
+            _call("vsv_adamw_read8", at, table.buffer_info()[0], len(part))
         return ms, vs
 
     def load_state_dict(self, state_dict):
@@ -134,7 +128,7 @@ class AdamW(torch.optim.Optimizer):
 
 
 def _check_param(p):
-    if str(p.dtype) not in _lib.VSV_DTYPES:
+    if p.dtype not in _TYPES:
         raise ValueError(f"AdamW: parameters must be float32, bfloat16 or float16, not {p.dtype}")
     if not p.is_contiguous():
         raise ValueError("AdamW: parameters must be contiguous")
@@ -142,13 +136,12 @@ def _check_param(p):
 
 def _table(rows, bits):
     """struct vsv_adamw_tensor[len(rows)] of (p, g, state) rows, as 64-bit words."""
-    t = np.zeros((len(rows), 7), dtype=np.uint64)
-    t[:, 0] = [p.data_ptr() for p, _, _ in rows]
-    t[:, 1] = [g.data_ptr() for _, g, _ in rows]
-    t[:, 2] = [st["exp_avg"].data_ptr() for _, _, st in rows]
-    t[:, 3] = [st["exp_avg_sq"].data_ptr() for _, _, st in rows]
-    if bits == 8:
-        t[:, 4] = [st["exp_avg_scale"].data_ptr() for _, _, st in rows]
-        t[:, 5] = [st["exp_avg_sq_scale"].data_ptr() for _, _, st in rows]
-    t[:, 6] = [p.numel() for p, _, _ in rows]
-    return t
+    words = []
+    for p, g, st in rows:
+        m = st["exp_avg"]
+        if bits == 8:
+            words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
+                      st["exp_avg_sq_scale"].data_ptr(), m.numel())
+        else:
+            words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), st["exp_avg_sq"].data_ptr(), 0, 0, m.numel())
+    return array.array("Q", words)

@@ -27,9 +27,14 @@ from . import lib as _lib
 _GPU = "there is no CPU fallback"
 
 
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}              # VSV_F32, VSV_BF16, VSV_F16
+_Tensor, _f32_type = torch.Tensor, torch.float32
+_entries = {}
+
+
 def _last(t):
     """t itself where its last dimension is contiguous, else a copy."""
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _ptr(t):
@@ -37,26 +42,26 @@ def _ptr(t):
 
 
 def _seq(what, name, t, shape, dtype=None):
-    if not torch.is_tensor(t) or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: {name} must be a tensor of shape {tuple(shape)}, not {tuple(t.shape) if torch.is_tensor(t) else t!r}")
-    if str(t.dtype) not in _lib.VSV_DTYPES or (dtype is not None and t.dtype != dtype):
+    if not isinstance(t, _Tensor) or t.shape != shape:
+        raise ValueError(f"{what}: {name} must be a tensor of shape {tuple(shape)}, not {tuple(t.shape) if isinstance(t, _Tensor) else t!r}")
+    if t.dtype not in _TYPES or (dtype is not None and t.dtype != dtype):
         raise ValueError(f"{what}: {name} must be {dtype or 'float32, bfloat16 or float16'}, not {t.dtype}")
-    return _last(t)
+    return t if t.is_contiguous() else _last(t)
 
 
 def _f32(what, name, t, shape):
     if t is None:
         return None
-    if not torch.is_tensor(t) or tuple(t.shape) != tuple(shape) or t.dtype != torch.float32:
+    if not isinstance(t, _Tensor) or t.shape != shape or t.dtype is not _f32_type:
         raise ValueError(f"{what}: {name} must be a float32 tensor of shape {tuple(shape)}"
-                         + (f", not {t.dtype} {tuple(t.shape)}" if torch.is_tensor(t) else f", not {t!r}"))
-    return t.contiguous()
+                         + (f", not {t.dtype} {tuple(t.shape)}" if isinstance(t, _Tensor) else f", not {t!r}"))
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _lengths(what, t, B):
     if t is None:
         return None
-    if not torch.is_tensor(t) or tuple(t.shape) != (B,) or t.dtype not in (torch.int32, torch.int64):
+    if not isinstance(t, _Tensor) or t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: lengths must be an int32 or int64 tensor of shape ({B},)")
     if t.dtype == torch.int64:
         t = t.clamp(0, 2**31 - 1).to(torch.int32)
@@ -66,26 +71,50 @@ def _lengths(what, t, B):
 def _same_gpu(what, x, *others):
     if not x.is_cuda:
         raise RuntimeError(f"{what}: tensors must be on a GPU; {_GPU}")
+    at = x.get_device()
     for t in others:
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != at:
             raise ValueError(f"{what}: tensors are on {t.device} and {x.device}")
 
 
-def _call(name, device, *args):
-    """One entry point on the device's current stream."""
-    fn = getattr(_lib.load(), name)
-    with torch.cuda.device(device):
-        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+def _call(name, at, *args):
+    """One entry point on the current stream of GPU `at`."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    if torch._C._cuda_getDevice() == at:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    else:
+        with torch.cuda.device(at):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
     if rc:
         _lib.check(rc, name)
 
 
+def _size(name, desc):
+    """A size that the library answers for a descriptor."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    return fn(desc)
+
+
 def _workspace(nbytes, device):
-    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes or 16, dtype=torch.uint8, device=device)
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if not torch.is_grad_enabled():
+        return False
+    for t in ts:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _touched(t):
+    """What an in-place operation leaves on a tensor that was written through its address."""
+    torch.autograd.graph.increment_version(t)
 
 
 # ---- short causal convolution ------------------------------------------------------------------------------------
@@ -96,10 +125,10 @@ def short_conv(x, weight, bias=None, *, silu=True, initial_state=None, lengths=N
     x (B, T, D), weight (D, K) with 1 to 4 taps, bias (D).  initial_state (B, K - 1, D): the inputs before the first (zeros
     without it).  Returns y (B, T, D) [, the last K - 1 inputs (B, K - 1, D) in float32]."""
     what = "short_conv"
-    if not torch.is_tensor(x) or x.dim() != 3:
+    if not isinstance(x, _Tensor) or x.dim() != 3:
         raise ValueError(f"{what}: x must be a tensor (B, T, D)")
     B, T, D = x.shape
-    if not torch.is_tensor(weight) or weight.dim() != 2 or not 1 <= weight.shape[1] <= _lib.VSV_CONV_MAX_TAPS or D < 1:
+    if not isinstance(weight, _Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= _lib.VSV_CONV_MAX_TAPS or D < 1:
         raise ValueError(f"{what}: weight must be a tensor (D, K) with 1 to {_lib.VSV_CONV_MAX_TAPS} taps")
     K = weight.shape[1]
     x = _seq(what, "x", x, (B, T, D))
@@ -118,11 +147,11 @@ def short_conv(x, weight, bias=None, *, silu=True, initial_state=None, lengths=N
 def conv_forward(x, weight, bias, state_in, lengths, silu, want_state):
     """The launch behind short_conv: (y, state | None, the descriptor vsv_short_conv_backward takes again)."""
     (B, T, D), K = x.shape, weight.shape[1]
-    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     state = torch.empty((B, K - 1, D), dtype=torch.float32, device=x.device) if want_state else None
-    d = _lib.VsvShortConv(_lib.VSV_DTYPES[str(x.dtype)], K, int(silu), B, T, D, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(),
+    d = _lib.VsvShortConv(_TYPES[x.dtype], K, int(silu), B, T, D, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(),
                           _ptr(bias), _ptr(state_in), _ptr(lengths), y.data_ptr(), _ptr(state) or None)
-    _call("vsv_short_conv", x.device, C.byref(d))
+    _call("vsv_short_conv", x.get_device(), C.byref(d))
     return y, state, d
 
 
@@ -130,10 +159,10 @@ def short_conv_step(x, state, weight, bias=None, *, silu=True):
     """short_conv for one new token of every row: x (B, D) -> y (B, D); state (B, K - 1, D), contiguous float32, is updated in
     place.  No gradients."""
     what = "short_conv_step"
-    if not torch.is_tensor(x) or x.dim() != 2:
+    if not isinstance(x, _Tensor) or x.dim() != 2:
         raise ValueError(f"{what}: x must be a tensor (B, D)")
     B, D = x.shape
-    if not torch.is_tensor(weight) or weight.dim() != 2 or not 1 <= weight.shape[1] <= _lib.VSV_CONV_MAX_TAPS or D < 1:
+    if not isinstance(weight, _Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= _lib.VSV_CONV_MAX_TAPS or D < 1:
         raise ValueError(f"{what}: weight must be a tensor (D, K) with 1 to {_lib.VSV_CONV_MAX_TAPS} taps")
     K = weight.shape[1]
     x = _seq(what, "x", x, (B, D))
@@ -142,38 +171,40 @@ def short_conv_step(x, state, weight, bias=None, *, silu=True):
     _same_gpu(what, x, weight, bias, state)
     if _wants_grad(x, weight, bias, state):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    d = _lib.VsvShortConv(_lib.VSV_DTYPES[str(x.dtype)], K, int(silu), B, 1, D, x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _ptr(bias),
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    d = _lib.VsvShortConv(_TYPES[x.dtype], K, int(silu), B, 1, D, x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _ptr(bias),
                           None, None, y.data_ptr(), state.data_ptr())
-    _call("vsv_short_conv_step", x.device, C.byref(d))
-    torch.autograd.graph.increment_version(state)
+    _call("vsv_short_conv_step", x.get_device(), C.byref(d))
+    _touched(state)
     return y
 
 
 def _in_place(what, state, shape):
-    if not torch.is_tensor(state) or tuple(state.shape) != tuple(shape) or state.dtype != torch.float32 or not state.is_contiguous():
+    if not isinstance(state, _Tensor) or state.shape != shape or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"{what}: state must be a contiguous float32 tensor of shape {tuple(shape)} (it is updated in place)")
 
 
 # ---- selective scan ----------------------------------------------------------------------------------------------
 
+def _grouped(what, name, t, lead, D, N, dtype):
+    """b or c with its group dimension."""
+    if isinstance(t, _Tensor) and t.dim() == len(lead) + 1:
+        t = t.unsqueeze(-2)
+    if not isinstance(t, _Tensor) or t.dim() != len(lead) + 2 or t.shape[-2] < 1 or D % t.shape[-2]:
+        raise ValueError(f"{what}: {name} must be a tensor ({', '.join(map(str, lead))}, [G,] N) with G a divisor of D = {D}")
+    return _seq(what, name, t, (*lead, t.shape[-2], N), dtype)
+
+
 def _scan_args(what, x, dt, a, b, c, skip, gate, dt_bias, lead):
     """The checked operands; b and c with their group dimension."""
     D = x.shape[-1]
-    if not torch.is_tensor(a) or a.dim() != 2 or a.shape[0] != D or not 1 <= a.shape[1] <= _lib.VSV_SSM_MAX_STATE or D < 1:
+    if not isinstance(a, _Tensor) or a.dim() != 2 or a.shape[0] != D or not 1 <= a.shape[1] <= _lib.VSV_SSM_MAX_STATE or D < 1:
         raise ValueError(f"{what}: a must be a tensor (D, N) with 1 to {_lib.VSV_SSM_MAX_STATE} states")
     N = a.shape[1]
     x = _seq(what, "x", x, (*lead, D))
     dt = _seq(what, "dt", dt, (*lead, D), x.dtype)
     gate = None if gate is None else _seq(what, "gate", gate, (*lead, D), x.dtype)
-    groups = []
-    for name, t in (("b", b), ("c", c)):
-        if torch.is_tensor(t) and t.dim() == len(lead) + 1:
-            t = t.unsqueeze(-2)
-        if not torch.is_tensor(t) or t.dim() != len(lead) + 2 or t.shape[-2] < 1 or D % t.shape[-2]:
-            raise ValueError(f"{what}: {name} must be a tensor ({', '.join(map(str, lead))}, [G,] N) with G a divisor of D = {D}")
-        groups.append(_seq(what, name, t, (*lead, t.shape[-2], N), x.dtype))
-    b, c = groups
+    b, c = _grouped(what, "b", b, lead, D, N, x.dtype), _grouped(what, "c", c, lead, D, N, x.dtype)
     if b.shape != c.shape:
         raise ValueError(f"{what}: b has {b.shape[-2]} groups and c {c.shape[-2]}")
     a, skip, dt_bias = _f32(what, "a", a, (D, N)), _f32(what, "skip", skip, (D,)), _f32(what, "dt_bias", dt_bias, (D,))
@@ -188,7 +219,7 @@ def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=Tru
 
     For gradients the states before every eighth step are kept (2 N bytes per element of x, in float32)."""
     what = "ssm_scan"
-    if not torch.is_tensor(x) or x.dim() != 3:
+    if not isinstance(x, _Tensor) or x.dim() != 3:
         raise ValueError(f"{what}: x must be a tensor (B, T, D)")
     B, T, D = x.shape
     x, dt, a, b, c, skip, gate, dt_bias = _scan_args(what, x, dt, a, b, c, skip, gate, dt_bias, (B, T))
@@ -199,35 +230,43 @@ def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=Tru
         from .autograd import SsmScan
         y, state = SsmScan.apply(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths, bool(softplus), bool(return_state))
     else:
-        y, state, _, _ = scan_forward(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths, softplus, return_state, False)
+        y, state, _, _ = scan_forward(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths, bool(softplus), return_state, False)
     return (y, state) if return_state else y
 
 
 def _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, state_in, lengths, softplus, B, T, y, state):
     D, N = a.shape
-    seq = T is not None                                                    # (B, D) rows have no time stride
-    ts = (lambda t: t.stride(1)) if seq else (lambda t: 0)
-    gs = lambda t: t.stride(-2)                                            # noqa: E731
-    return _lib.VsvSsm(_lib.VSV_DTYPES[str(x.dtype)], N, int(softplus), B, T if seq else 1, D, b.shape[-2],
-                       x.data_ptr(), x.stride(0), ts(x), dt.data_ptr(), dt.stride(0), ts(dt),
-                       _ptr(gate), 0 if gate is None else gate.stride(0), 0 if gate is None else ts(gate),
-                       b.data_ptr(), b.stride(0), ts(b), gs(b), c.data_ptr(), c.stride(0), ts(c), gs(c),
+    if T is not None:
+        x_bs, x_ts, _ = x.stride()
+        dt_bs, dt_ts, _ = dt.stride()
+        g_bs, g_ts, _ = gate.stride() if gate is not None else (0, 0, 0)
+        b_bs, b_ts, b_gs, _ = b.stride()
+        c_bs, c_ts, c_gs, _ = c.stride()
+    else:                                                                  # (B, D) rows: one step, no time stride
+        T = 1
+        x_bs, x_ts, dt_bs, dt_ts, b_ts, c_ts, g_ts = x.stride(0), 0, dt.stride(0), 0, 0, 0, 0
+        g_bs = gate.stride(0) if gate is not None else 0
+        b_bs, b_gs, _ = b.stride()
+        c_bs, c_gs, _ = c.stride()
+    return _lib.VsvSsm(_TYPES[x.dtype], N, softplus, B, T, D, b.shape[-2], x.data_ptr(), x_bs, x_ts, dt.data_ptr(), dt_bs, dt_ts,
+                       _ptr(gate), g_bs, g_ts, b.data_ptr(), b_bs, b_ts, b_gs, c.data_ptr(), c_bs, c_ts, c_gs,
                        a.data_ptr(), _ptr(skip), _ptr(dt_bias), _ptr(state_in), _ptr(lengths), y.data_ptr(), _ptr(state), None)
 
 
 def scan_forward(x, dt, a, b, c, skip, gate, dt_bias, state_in, lengths, softplus, want_state, save):
     """The launches behind ssm_scan: (y, state | None, the descriptor vsv_ssm_scan_backward takes again, saved | None)."""
     (B, T, D), N = x.shape, a.shape[1]
-    y = torch.empty((B, T, D), dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     state = torch.empty((B, D, N), dtype=torch.float32, device=x.device) if want_state else None
     d = _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, state_in, lengths, softplus, B, T, y, state)
-    lib = _lib.load()
+    ref = C.byref(d)
     saved = None
     if save:
-        saved = torch.empty(lib.vsv_ssm_saved_floats(C.byref(d)), dtype=torch.float32, device=x.device)
-        d.saved = _ptr(saved) or None
-    ws = _workspace(lib.vsv_ssm_scan_ws_bytes(C.byref(d)), x.device)
-    _call("vsv_ssm_scan", x.device, C.byref(d), ws.data_ptr(), ws.numel())
+        saved = torch.empty(_size("vsv_ssm_saved_floats", ref), dtype=torch.float32, device=x.device)
+        d.saved = saved.data_ptr() or None
+    nbytes = _size("vsv_ssm_scan_ws_bytes", ref)
+    ws = _workspace(nbytes, x.device) if nbytes else None
+    _call("vsv_ssm_scan", x.get_device(), ref, _ptr(ws), nbytes)
     return y, state, d, saved
 
 
@@ -235,7 +274,7 @@ def ssm_step(x, dt, a, b, c, skip=None, gate=None, *, state, dt_bias=None, softp
     """ssm_scan for one new token of every row: x, dt [, gate] (B, D), b, c (B, [G,] N) -> y (B, D); state (B, D, N),
     contiguous float32, is updated in place.  No gradients."""
     what = "ssm_step"
-    if not torch.is_tensor(x) or x.dim() != 2:
+    if not isinstance(x, _Tensor) or x.dim() != 2:
         raise ValueError(f"{what}: x must be a tensor (B, D)")
     B, D = x.shape
     x, dt, a, b, c, skip, gate, dt_bias = _scan_args(what, x, dt, a, b, c, skip, gate, dt_bias, (B,))
@@ -243,10 +282,10 @@ def ssm_step(x, dt, a, b, c, skip=None, gate=None, *, state, dt_bias=None, softp
     _same_gpu(what, x, dt, a, b, c, skip, gate, dt_bias, state)
     if _wants_grad(x, dt, a, b, c, skip, gate, dt_bias, state):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    d = _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, None, None, softplus, B, None, y, state)
-    _call("vsv_ssm_step", x.device, C.byref(d))
-    torch.autograd.graph.increment_version(state)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    d = _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, None, None, bool(softplus), B, None, y, state)
+    _call("vsv_ssm_step", x.get_device(), C.byref(d))
+    _touched(state)
     return y
 
 
