@@ -111,6 +111,35 @@ def test_8_bits(dtype):
         assert torch.equal(v.cpu().reshape(-1), (st["exp_avg_sq_scale"].cpu().double()[block] * tv[q]).float())
 
 
+def test_8_bits_moments_are_the_formulas_bit_for_bit():
+    """The same bfloat16 gradients twice (few mantissas, so sums that lie next to the middle between two float32 scales are common):
+    after either step every moment read back equals the formulas in 64 bits, products and sums rounded one by one."""
+    from vsv.optim import AdamW
+    g = torch.Generator().manual_seed(9)
+    n = 256 * 2000 + 77
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+    opt = AdamW([p], state_bits=8)
+    p.grad = (torch.randn(n, generator=g) * torch.exp(2 * torch.randn(n, generator=g)) * 1e-3).to(torch.bfloat16).cuda()
+    gr, block = p.grad.double().cpu(), torch.arange(n) // 256
+    tm, tv = (torch.arange(128).double() / 127) ** 2, (torch.arange(256).double() / 255) ** 4
+    m, v = torch.zeros(n).double(), torch.zeros(n).double()
+    for t in (1, 2):
+        opt.step()
+        m, v = m * 0.9 + gr * (1 - 0.9), v * 0.999 + gr * gr * (1 - 0.999)
+        u = (((torch.arange(n) * 0xC13FA9A9 % 2**32) + t * 0x91E10DA5) % 2**32).double().add(0.5) / 2**32
+        new = []
+        for x, table, share in ((m, tm, u), (v, tv, 1 - u)):
+            top = torch.zeros(2001).double().scatter_reduce_(0, block, x.abs(), "amax").float().double()[block]
+            k, near = _codes(x.abs(), table, top, share)
+            assert near.min() > 1e-11                                        # (no share of these inputs is closer to its threshold)
+            if table is tv:
+                k = torch.where((k < 1) & (x > 0), 1, k)
+            new.append((torch.sign(x) * top * table[k]).float().double())
+        m, v = new
+        got_m, got_v = opt.moments()
+        assert (got_m[0].double().cpu() != m).sum() == 0 and (got_v[0].double().cpu() != v).sum() == 0
+
+
 def test_8_bits_do_not_lose_small_changes():
     """v under gradients of one size: after 700 steps its mean over elements is 1 - 0.999^700 = 0.5036 g^2.  A dither that is even over
     steps and elements keeps the mean's error below half a code step (4 / 255 / 2 = 0.8 %); rounding to the nearest code would freeze it."""

@@ -98,6 +98,17 @@ __device__ inline float read_v8(unsigned k, double s) {
     return (float)(k2 * k2 * s);
 }
 
+// The moments as the formulas write them, operation by operation: gradients of 16 bits have so few mantissas that a sum next
+// to the middle between two float32 scales is no rarity, and a fused sum fell on the other side of it in 0.8 % of the blocks.
+__device__ inline double next_m(double m, double g, const Hyper& h) {
+#pragma clang fp contract(off)
+    return m * h.b1d + g * h.w1d;
+}
+__device__ inline double next_v(double v, double g, const Hyper& h) {
+#pragma clang fp contract(off)
+    return v * h.b2d + g * g * h.w2d;
+}
+
 // The codes by the definition, in 64 bits.
 __device__ inline int exact_m8(double x, double inv, double u) {
     const double y = fmin(fabs(x) * inv, kFullM);
@@ -161,8 +172,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hype
 #pragma unroll
     for (int j = 0; j < kPer8; ++j) {
         const double gd = gv[j];
-        m[j] = __builtin_fma(gd, h.w1d, (double)read_m8(mk.v[j], ms) * h.b1d);
-        v[j] = __builtin_fma(gd * gd, h.w2d, (double)read_v8(vk.v[j], vs) * h.b2d);
+        m[j] = next_m(read_m8(mk.v[j], ms), gd, h);
+        v[j] = next_v(read_v8(vk.v[j], vs), gd, h);
         finite = __builtin_fmaf(gv[j], 0.0f, finite);
     }
     if (finite != 0.0f) {                                                 // some gradient here is not finite

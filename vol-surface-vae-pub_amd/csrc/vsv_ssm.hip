@@ -983,7 +983,7 @@ long ssm_blocks(const vsv_ssm_desc* a) { return (a->D / a->G + 63) / 64; }
 // The scan's split of time.  A split costs a second pass (1.8 times the work) and a launch, so it pays below half a wave per
 // SIMD (1024 of them) and from kSplitFrom steps on: then as many segments as make two waves per SIMD, none shorter than two
 // tiles, at most kMaxSegments (the start of a segment walks over those in front of it).
-constexpr long kMaxSegments = 64, kSplitFrom = 128, kSplitWaves = 2048;
+constexpr long kMaxSegments = 64, kSplitFrom = 64, kSplitWaves = 2048;
 
 ScanPlan scan_plan(const vsv_ssm_desc* a) {
     ScanPlan pl = {};
