@@ -110,38 +110,53 @@ __device__ inline double next_v(double v, double g, const Hyper& h) {
 }
 
 // The codes by the definition, in 64 bits.
-__device__ inline int exact_m8(double x, double inv, double u) {
-    const double y = fmin(fabs(x) * inv, kFullM);
+__device__ inline int exact_m8(double x, double scale, double u) {
+    const double y = fmin(fabs(x) / scale * kFullM, kFullM);
     double k = (double)(int)__builtin_amdgcn_sqrtf((float)y);
     if (k * k > y) k -= 1.0;
     if ((k + 1.0) * (k + 1.0) <= y) k += 1.0;
     return (int)k + (y - k * k > u * (2.0 * k + 1.0));
 }
-__device__ inline int exact_v8(double x, double inv, double u) {
-    const double y = fmin(x * inv, kFullV);
+__device__ inline int exact_v8(double x, double scale, double u) {
+    const double y = fmin(x / scale * kFullV, kFullV);
     double k = (double)(int)__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y));
     double k2 = k * k, up = (k + 1.0) * (k + 1.0);
     if (k2 * k2 > y) { up = k2; k -= 1.0; k2 = k * k; }
     if (up * up <= y) { k2 = up; k += 1.0; up = (k + 1.0) * (k + 1.0); }
     return (int)k + (y - k2 * k2 > u * (up * up - k2 * k2));
 }
-// The same in float32, where no more than 2e-5 of a gap is lost: `near` is set where the value lies that close to its
-// threshold, and the 64-bit form decides there.  Next to a code's own value k may come out one off, the share of the gap
-// then next to 1 for next to 0 or the other way round: the code is the same for any u but those next to 0 and 1, which the
-// caller counts as near.
+// The same in float32 (a code as a float), where no more than 3e-5 of a gap is lost: `least` is the smallest distance to a
+// threshold, in gaps less kNear, and the 64-bit form decides where it is negative.  Next to a code's own value k may come out
+// one off, the share of the gap then next to 1 for next to 0 or the other way round: the code is the same for any u but those
+// next to 0 and 1, which the caller counts as near.
 constexpr float kNear = 1e-4f;
-__device__ inline int code_m8(float x, float inv, float u, bool& near) {
+__device__ inline float step_up(float over) { return __builtin_amdgcn_fmed3f(over * 1e30f, 0.0f, 1.0f); }
+__device__ inline float code_m8(float x, float inv, float u, float& least) {
     const float y = __builtin_fabsf(x) * inv, k = floorf(__builtin_amdgcn_sqrtf(y));
     const float gap = __builtin_fmaf(2.0f, k, 1.0f), over = __builtin_fmaf(-u, gap, __builtin_fmaf(-k, k, y));
-    near |= __builtin_fabsf(over) < kNear * gap;
-    return (int)k + (over > 0.0f);
+    least = __builtin_fminf(least, __builtin_fmaf(-kNear, gap, __builtin_fabsf(over)));
+    return k + step_up(over);
 }
-__device__ inline int code_v8(float x, float inv, float u, bool& near) {
+__device__ inline float code_v8(float x, float inv, float u, float& least) {
     const float y = x * inv, k = floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(y))), k2 = k * k;
-    const float gap = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(4.0f, k, 6.0f), k, 4.0f), k, 1.0f);
+    const float d = __builtin_fmaf(2.0f, k, 1.0f), gap = d * __builtin_fmaf(2.0f, k2, d);         // (k+1)^4 - k^4
     const float over = __builtin_fmaf(-u, gap, __builtin_fmaf(-k2, k2, y));
-    near |= __builtin_fabsf(over) < kNear * gap;
-    return (int)k + (over > 0.0f);
+    least = __builtin_fminf(least, __builtin_fmaf(-kNear, gap, __builtin_fabsf(over)));
+    return k + step_up(over);
+}
+
+// The largest of the 32 lanes that share a block.
+template <int CTRL> __device__ inline float max_dpp(float v) {
+    return __builtin_fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)));
+}
+__device__ inline float block_max(float v) {
+    v = max_dpp<0xb1>(v);                                                 // lanes 1, 2, 7 - l, 15 - l apart
+    v = max_dpp<0x4e>(v);
+    v = max_dpp<0x141>(v);
+    v = max_dpp<0x140>(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned r0 = r[0], r1 = r[1];                                  // and the neighbouring sixteen
+    return __builtin_fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
 }
 
 template <typename T>
@@ -177,6 +192,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hype
         finite = __builtin_fmaf(gv[j], 0.0f, finite);
     }
     if (finite != 0.0f) {                                                 // some gradient here is not finite
+        asm volatile("");                                                 // (a branch: the selects would cost every step six operations an element)
 #pragma unroll
         for (int j = 0; j < kPer8; ++j)
             if (!__builtin_isfinite(gv[j])) { m[j] = read_m8(mk.v[j], ms); v[j] = read_v8(vk.v[j], vs); pv[j] = __builtin_nanf(""); }
@@ -189,37 +205,41 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hype
         v32[j] = (float)v[j];
         sm = __builtin_fmaxf(sm, __builtin_fabsf(m32[j]));
         sv = __builtin_fmaxf(sv, v32[j]);
-        // the fast root and reciprocal, an ulp each; without an eps subnormal second moments would count, which they lose
-        float den = __builtin_fmaf(__builtin_amdgcn_sqrtf(v32[j]), h.inv_root, h.eps);
-        if (h.eps < 1e-15f) den = __builtin_fmaf((float)sqrt(v[j]), h.inv_root, h.eps);
-        pv[j] = __builtin_fmaf(-h.rate * m32[j], __builtin_amdgcn_rcpf(den), pv[j] * h.decay);
     }
+    // (the fast root and reciprocal, an ulp each; without an eps subnormal second moments would count, which they lose)
+    if (h.eps >= 1e-15f) {
 #pragma unroll
-    for (int w = kLanes8 / 2; w > 0; w >>= 1) {
-        sm = __builtin_fmaxf(sm, __shfl_xor(sm, w, kLanes8));
-        sv = __builtin_fmaxf(sv, __shfl_xor(sv, w, kLanes8));
+        for (int j = 0; j < kPer8; ++j)
+            pv[j] = __builtin_fmaf(-h.rate * m32[j], __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_sqrtf(v32[j]), h.inv_root, h.eps)),
+                                   pv[j] * h.decay);
+    } else {
+        asm volatile("");
+#pragma unroll
+        for (int j = 0; j < kPer8; ++j) pv[j] = pv[j] * h.decay - h.rate * (float)(m[j] / (sqrt(v[j]) * h.inv_root + h.eps));
     }
-    sm = __builtin_fminf(sm, FLT_MAX);
-    sv = __builtin_fminf(sv, FLT_MAX);
-    const double im = sm > 0.0f ? kFullM / (double)sm : 0.0, iv = sv > 0.0f ? kFullV / (double)sv : 0.0;
+    sm = __builtin_fminf(block_max(sm), FLT_MAX);
+    sv = __builtin_fminf(block_max(sv), FLT_MAX);
     // (float32 holds neither factor where the scale is next to its limits: there, all codes by the definition)
     const bool plain = (sm > 0.0f && (sm < 1e-30f || sm > 1e30f)) || (sv > 0.0f && (sv < 1e-26f || sv > 1e30f));
-    const float im32 = (float)im, iv32 = (float)iv;
+    const float im = sm > 0.0f ? (float)kFullM * __builtin_amdgcn_rcpf(sm) : 0.0f, iv = sv > 0.0f ? (float)kFullV * __builtin_amdgcn_rcpf(sv) : 0.0f;
+    const unsigned some = sv > 0.0f;
 #pragma unroll
     for (int j = 0; j < kPer8; ++j) {
         const unsigned weyl = (unsigned)(o + j) * VSV_ADAMW_WEYL_I + h.dither;
         const float u = (float)weyl * 0x1p-32f;
-        bool near = plain || __builtin_fabsf(u - 0.5f) > 0.5f - kNear;
-        int km = code_m8(m32[j], im32, u, near), kv = code_v8(v32[j], iv32, 1.0f - u, near);
-        if (near) {
+        float least = plain ? -1.0f : 0.5f - kNear - __builtin_fabsf(u - 0.5f);
+        const float km = code_m8(m32[j], im, u, least), kv = code_v8(v32[j], iv, 1.0f - u, least);
+        int cm = (int)__builtin_copysignf(km, m32[j]), cv = (int)kv;
+        if (!(least >= 0.0f)) {
             const double ud = ((double)weyl + 0.5) * 0x1p-32;
-            km = exact_m8(m[j], im, ud);
-            kv = exact_v8(v[j], iv, 1.0 - ud);
+            cm = sm > 0.0f ? exact_m8(m[j], sm, ud) : 0;
+            cm = m[j] < 0.0 ? -cm : cm;
+            cv = sv > 0.0f ? exact_v8(v[j], sv, 1.0 - ud) : 0;
         }
-        const int least = v[j] > 0.0 && sv > 0.0f;
-        kv = kv > least ? kv : least;
-        mk.v[j] = (int8_t)(m32[j] < 0.0f ? -km : km);
-        vk.v[j] = (uint8_t)kv;
+        // v > 0 (its upper word, then, is not 0) never gets code 0
+        const unsigned high = (unsigned)(__builtin_bit_cast(unsigned long long, v[j]) >> 32), one = high < some ? high : some;
+        mk.v[j] = (int8_t)cm;
+        vk.v[j] = (uint8_t)((unsigned)cv > one ? (unsigned)cv : one);
     }
     if (wide) {
         store_vec<T, kPer8>(p + o, pv);
