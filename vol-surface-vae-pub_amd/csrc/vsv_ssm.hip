@@ -34,7 +34,7 @@ __device__ inline float conv_silu(float s) {
 // One read of x and one write of y (2K flops an element): bound by memory.  A thread owns VEC neighbouring channels and a
 // chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it works on kRows rows at a
 // time, with the next ones under way.
-constexpr int kRows = 4;
+constexpr int kRows = 4, kConvVec = 4;
 
 template <typename T, int K, int VEC> struct ConvRows {
     const T* x;                      // the sequence's row 0, at this thread's channels
@@ -928,22 +928,26 @@ int check_conv(const vsv_short_conv_desc* a, const char* what) {
     return 0;
 }
 
-// 16 bytes per access where every row starts on them
-bool conv_wide(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, size_t size, long vec) {
-    bool ok = a->D % vec == 0 && a->x_bs % vec == 0 && a->x_ts % vec == 0 && aligned(a->x, vec * size) && aligned(a->y, vec * size);
-    if (g) ok = ok && g->dy_bs % vec == 0 && g->dy_ts % vec == 0 && aligned(g->dy, vec * size) && aligned(g->dx, vec * size);
+// Four channels per access where every row starts on such a word (eight in 16 bits need all registers in the backward pass and
+// gain nothing in the forward one).
+bool conv_wide(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, size_t size) {
+    constexpr long v = kConvVec;
+    bool ok = a->D % v == 0 && a->x_bs % v == 0 && a->x_ts % v == 0 && aligned(a->x, v * size) && aligned(a->y, v * size);
+    if (g) ok = ok && g->dy_bs % v == 0 && g->dy_ts % v == 0 && aligned(g->dy, v * size) && aligned(g->dx, v * size);
     return ok;
 }
 
-// Time steps per thread: the longer, the less is read twice and the fewer sums are left over, as long as there are two waves
-// for every SIMD (131072 threads).
-long conv_chunk(const vsv_short_conv_desc* a) {
-    const long vecs = a->D / (a->D % 8 == 0 ? 8 : 1), rows = a->B * vecs;
+// Time steps per thread: the longer, the less is read twice and the fewer sums are left over, as long as the threads fill the
+// chip.  Forward eight waves for every SIMD (8x2048x4096 bf16: two 87, four 77, eight 74 us); backward, where a chunk leaves K + 1
+// sums per channel, two (131 us, four 138).
+constexpr long kConvFill = 524288, kConvBwdFill = 131072;
+long conv_chunk(const vsv_short_conv_desc* a, long fill) {
+    const long rows = a->B * (a->D / (a->D % kConvVec == 0 ? kConvVec : 1));
     long chunk = 16;
-    while (chunk < 256 && rows * ((a->T + 2 * chunk - 1) / (2 * chunk)) >= 131072) chunk *= 2;
+    while (chunk < 256 && rows * ((a->T + 2 * chunk - 1) / (2 * chunk)) >= fill) chunk *= 2;
     return chunk;
 }
-long conv_chunks(const vsv_short_conv_desc* a) { const long c = conv_chunk(a); return a->T > 0 ? (a->T + c - 1) / c : 1; }
+long conv_chunks(const vsv_short_conv_desc* a, long fill) { const long c = conv_chunk(a, fill); return a->T > 0 ? (a->T + c - 1) / c : 1; }
 
 template <typename F> int by_taps(int K, F&& f) {
     switch (K) {
@@ -1016,12 +1020,12 @@ extern "C" int vsv_short_conv(const vsv_short_conv_desc* a, void* stream) {
     return by_dtype(a->dtype, "vsv_short_conv", [&](auto t) {
         using T = decltype(t);
         return by_taps(a->K, [&](auto k) {
-            constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
-            const bool wide = conv_wide(a, nullptr, sizeof(T), V);
-            const long nc = conv_chunks(a), nv = wide ? a->D / V : a->D, blocks = (a->B * nc * nv + 255) / 256;
+            constexpr int K = decltype(k)::value;
+            const bool wide = conv_wide(a, nullptr, sizeof(T));
+            const long nc = conv_chunks(a, kConvFill), nv = wide ? a->D / kConvVec : a->D, blocks = (a->B * nc * nv + 255) / 256;
             if (blocks > kMaxBlocks) { set_error("vsv_short_conv: too many elements for one call"); return -2; }
-            if (wide) hipLaunchKernelGGL((short_conv_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a), nc, nv);
-            else hipLaunchKernelGGL((short_conv_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a), nc, nv);
+            if (wide) hipLaunchKernelGGL((short_conv_kernel<T, K, kConvVec>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a, kConvFill), nc, nv);
+            else hipLaunchKernelGGL((short_conv_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a, kConvFill), nc, nv);
             return op_launch_check("short_conv_kernel");
         });
     });
@@ -1029,24 +1033,24 @@ extern "C" int vsv_short_conv(const vsv_short_conv_desc* a, void* stream) {
 
 extern "C" size_t vsv_short_conv_backward_ws_bytes(const vsv_short_conv_desc* a) {
     if (check_conv(a, "vsv_short_conv_backward_ws_bytes")) return 0;
-    return (size_t)a->B * conv_chunks(a) * (a->K + 1) * a->D * sizeof(float);
+    return (size_t)a->B * conv_chunks(a, kConvBwdFill) * (a->K + 1) * a->D * sizeof(float);
 }
 
 extern "C" int vsv_short_conv_backward(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = check_conv(a, "vsv_short_conv_backward")) return rc;
     if (!g || (a->B > 0 && a->T > 0 && (!g->dy || !g->dx))) { set_error("vsv_short_conv_backward: null pointer"); return -1; }
     if (ws_bytes < vsv_short_conv_backward_ws_bytes(a) || (!ws && a->B > 0)) { set_error("vsv_short_conv_backward: workspace too small"); return -1; }
-    const long nc = conv_chunks(a), M = (a->K + 1) * a->D;
+    const long nc = conv_chunks(a, kConvBwdFill), M = (a->K + 1) * a->D;
     if (a->B > 0) {
         const int rc = by_dtype(a->dtype, "vsv_short_conv_backward", [&](auto t) {
             using T = decltype(t);
             return by_taps(a->K, [&](auto k) {
-                constexpr int K = decltype(k)::value, V = 4;              // (eight channels a thread would need all its registers)
-                const bool wide = conv_wide(a, g, sizeof(T), V);
-                const long nv = wide ? a->D / V : a->D, blocks = (a->B * nc * nv + 255) / 256;
+                constexpr int K = decltype(k)::value;
+                const bool wide = conv_wide(a, g, sizeof(T));
+                const long nv = wide ? a->D / kConvVec : a->D, blocks = (a->B * nc * nv + 255) / 256;
                 if (blocks > kMaxBlocks) { set_error("vsv_short_conv_backward: too many elements for one call"); return -2; }
-                if (wide) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a), nc, nv, (float*)ws);
-                else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a), nc, nv, (float*)ws);
+                if (wide) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, kConvVec>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a, kConvBwdFill), nc, nv, (float*)ws);
+                else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a, kConvBwdFill), nc, nv, (float*)ws);
                 return op_launch_check("short_conv_bwd_kernel");
             });
         });
