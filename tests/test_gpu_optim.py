@@ -248,6 +248,32 @@ def test_state_dict_groups_and_missing_gradients(bits):
     assert all(torch.equal(p, q) for p, q in zip(ps, twins))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_and_what_does_not_fit(bits):
+    """A deep copy steps like the original; a parameter that has changed its size, and saved state of another shape, are refused
+    before anything is launched."""
+    import copy
+    from vsv.optim import AdamW
+    p = torch.nn.Parameter(torch.randn(300, device="cuda"))
+    opt = AdamW([p], state_bits=bits)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    q, twin = copy.deepcopy((p, opt))
+    q.grad = p.grad.clone()
+    twin.param_groups[0]["params"][0].grad = p.grad.clone()
+    opt.step(); twin.step()
+    assert torch.equal(p, twin.param_groups[0]["params"][0]) and twin.state_bits == bits
+    big = torch.nn.Parameter(torch.zeros(600, device="cuda"))
+    with pytest.raises(ValueError, match="exp_avg"):
+        AdamW([big], state_bits=bits).load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError, match="bits"):
+        AdamW([p], state_bits=40 - bits).load_state_dict(opt.state_dict())
+    p.data = torch.zeros(600, device="cuda")
+    p.grad = torch.zeros(600, device="cuda")
+    with pytest.raises(ValueError, match="shape"):
+        opt.step()
+
+
 def test_closure_scheduler_and_capture():
     from vsv.optim import AdamW
     p = torch.nn.Parameter(torch.ones(10, device="cuda"))

@@ -104,6 +104,22 @@ def test_scan_padded(T, lengths, dtype):
     assert all(torch.equal(got[k], again[k]) for k in got)
 
 
+def test_scan_one_step_whatever_its_stride():
+    """A single step's time stride is of no account, however large."""
+    s = _scan_case(14, 3, 1, 65, 16, 1, "fp32")
+    want = _scan_run(s)
+    v = dict(s)
+    for n in ("x", "dt", "gate"):
+        v[n] = torch.as_strided(s[n], (3, 1, 65), (65, 2**40, 1))
+    got = _scan_run(v)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    wide = torch.zeros(1, device="cuda").expand(2, 2**27)                                # two steps of 2^27 channels: refused, not wrapped
+    from vsv.ssm import ssm_scan
+    with pytest.raises(ValueError, match="channels"):
+        ssm_scan(wide.unsqueeze(0), wide.unsqueeze(0), torch.zeros(1, 1, device="cuda").expand(2**27, 1), torch.zeros(1, 2, 1, device="cuda"),
+                 torch.zeros(1, 2, 1, device="cuda"))
+
+
 def test_scan_of_nothing():
     for B, T in ((2, 0), (0, 5), (0, 0)):
         s = _scan_case(6, B, T, 40, 16, 1, "fp32")

@@ -126,6 +126,12 @@ def test_optimizer_refuses():
     p.grad = torch.zeros(4, 3).to_sparse()
     with pytest.raises(ValueError, match="gradient"):
         opt.step()
+    with pytest.raises(ValueError, match="same number of bits"):
+        AdamW([{"params": [p], "state_bits": 8}])
+    from vsv.ssm import SsmMemory
+    for bad in (dict(state_size=17), dict(state_size=0), dict(taps=5)):
+        with pytest.raises(ValueError, match="are built"):
+            SsmMemory(4, 8, **bad)
     with pytest.raises(ValueError, match="8 bits"):
         AdamW([p], state_bits=8).load_state_dict({"state": {0: {"step": 1, "exp_avg": torch.zeros(4, 3)}}, "param_groups": opt.state_dict()["param_groups"]})
 
@@ -142,6 +148,8 @@ def test_c_entries_check_their_arguments():
     g = vlib.VsvShortConvGrads(dy=16, dx=16)
     assert L.vsv_short_conv_backward(C.byref(conv()), C.byref(g), None, 0, None) == -1 and b"workspace" in L.vsv_last_error()
     assert L.vsv_short_conv_step(C.byref(conv()), None) == -1                                  # (no state)
+    for bad in (scan(x_ts=2**26), scan(gate=16, gate_ts=-1), scan(D=2**26)):
+        assert L.vsv_ssm_scan(C.byref(bad), None, 0, None) == -2 and b"stride" in L.vsv_last_error()
     for bad in (scan(N=0), scan(N=17), scan(G=3), scan(G=0), scan(B=-1), scan(T=-1), scan(D=0), scan(dtype=-1), scan(a=None), scan(x=None),
                 scan(c=None), scan(y=None)):
         assert L.vsv_ssm_scan(C.byref(bad), None, 0, None) == -1 and L.vsv_last_error()

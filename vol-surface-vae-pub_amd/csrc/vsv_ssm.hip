@@ -964,9 +964,9 @@ int check_ssm(const vsv_ssm_desc* a, const char* what) {
     if (a->B < 0 || a->T < 0 || a->D < 1) { set_error("%s: bad sizes (B %ld, T %ld, D %ld)", what, a->B, a->T, a->D); return -1; }
     if (a->G < 1 || a->D % a->G) { set_error("%s: %ld channels do not divide into %ld groups", what, a->D, a->G); return -1; }
     if (a->dtype < VSV_F32 || a->dtype > VSV_F16) { set_error("%s: dtype must be VSV_F32, VSV_BF16 or VSV_F16", what); return -1; }
-    const long most = 0x7fffffffL / (4 * 8);                             // (the scan addresses eight rows with 32 bits)
-    if (a->D > most || a->x_ts > most || a->dt_ts > most || a->gate_ts > most || a->x_ts < 0 || a->dt_ts < 0 || a->gate_ts < 0) {
-        set_error("%s: a time stride of more than %ld elements, or a negative one", what, most); return -2;
+    const long most = 0x7fffffffL / (4 * kTile);                          // (a tile's rows are addressed with 32 bits)
+    if (a->D > most || (a->T > 1 && (a->x_ts > most || a->dt_ts > most || a->gate_ts > most || a->x_ts < 0 || a->dt_ts < 0 || a->gate_ts < 0))) {
+        set_error("%s: more than %ld channels, or a time stride of more elements than that", what, most); return -2;
     }
     if (!a->a || (a->B > 0 && a->T > 0 && (!a->x || !a->dt || !a->b || !a->c || !a->y))) { set_error("%s: null pointer", what); return -1; }
     return 0;
@@ -1124,7 +1124,7 @@ extern "C" int vsv_ssm_scan_backward(const vsv_ssm_desc* a, const vsv_ssm_grads*
     if (!g || (a->B > 0 && a->T > 0 && (!a->saved || !g->dy || !g->dx || !g->ddt || !g->db || !g->dc || (a->gate && !g->dgate)))) {
         set_error("vsv_ssm_scan_backward: null pointer"); return -1;
     }
-    if (g->dy_ts < 0 || g->dy_ts > 0x7fffffffL / (4 * 8)) { set_error("vsv_ssm_scan_backward: bad time stride of dy"); return -2; }
+    if (a->T > 1 && (g->dy_ts < 0 || g->dy_ts > 0x7fffffffL / (4 * kTile))) { set_error("vsv_ssm_scan_backward: bad time stride of dy"); return -2; }
     if (ws_bytes < vsv_ssm_scan_backward_ws_bytes(a) || (a->B > 0 && (!ws || !aligned(ws, 16)))) {
         set_error("vsv_ssm_scan_backward: workspace too small or not on 16 bytes"); return -1;
     }

@@ -28,8 +28,11 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, not {state_bits!r}")
-        self.state_bits = state_bits
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    @property
+    def state_bits(self):
+        return self.defaults["state_bits"]                                 # (kept there, so copies and pickles have it)
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -38,25 +41,25 @@ class AdamW(torch.optim.Optimizer):
             lr, (b1, b2), eps, wd = float(g["lr"]), g["betas"], g["eps"], g["weight_decay"]
             if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and wd >= 0.0):
                 raise ValueError(f"AdamW: bad hyper-parameters lr={lr} betas={g['betas']} eps={eps} weight_decay={wd}")
+            if g["state_bits"] != self.state_bits:
+                raise ValueError("AdamW: all groups hold their moments in the same number of bits")
             for p in g["params"]:
                 _check_param(p)
         except Exception:
             self.param_groups.pop()
             raise
 
-    def _init_state(self, p):
-        st = self.state[p]
-        st["step"] = 0
+    def _layout(self, p):
+        """name -> (shape, type) of a parameter's state tensors."""
         if self.state_bits == 32:
-            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-        else:
-            blocks = -(-p.numel() // _lib.VSV_ADAMW_BLOCK)
-            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.int8, device=p.device)
-            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
-            st["exp_avg_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-            st["exp_avg_sq_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-        return st
+            return {"exp_avg": (p.shape, torch.float32), "exp_avg_sq": (p.shape, torch.float32)}
+        blocks = (-(-p.numel() // _lib.VSV_ADAMW_BLOCK),)
+        return {"exp_avg": (p.shape, torch.int8), "exp_avg_sq": (p.shape, torch.uint8),
+                "exp_avg_scale": (blocks, torch.float32), "exp_avg_sq_scale": (blocks, torch.float32)}
+
+    def _init_state(self, p):
+        self.state[p] = {"step": 0, **{k: torch.zeros(shape, dtype=dtype, device=p.device) for k, (shape, dtype) in self._layout(p).items()}}
+        return self.state[p]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -78,6 +81,9 @@ class AdamW(torch.optim.Optimizer):
                 if not p.is_cuda:
                     raise RuntimeError("AdamW: parameters must be on a GPU; there is no CPU fallback")
                 st = state[p] or self._init_state(p)
+                m = st["exp_avg"]
+                if m.shape != p.shape or m.get_device() != p.get_device():
+                    raise ValueError("AdamW: a parameter has changed its shape or device since its state was made")
                 rows.setdefault((p.dtype, p.get_device(), st["step"]), []).append((p, g if g.is_contiguous() else g.contiguous(), st))
             calls += [(group, *key, rows[key]) for key in rows]
         if calls and torch.cuda.is_current_stream_capturing():
@@ -112,19 +118,24 @@ class AdamW(torch.optim.Optimizer):
         return ms, vs
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the moments keep their own types (torch's casts floating state to the parameter's)."""
+        """As torch's, but the moments keep their own types (torch's casts floating state to the parameter's), and nothing that
+        does not fit the parameters is taken."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, st in state_dict["state"].items():
-            if ("exp_avg_scale" in st) != (self.state_bits == 8):
-                raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
-        super().load_state_dict(state_dict)
         params = [p for g in self.param_groups for p in g["params"]]
+        if any(g.get("state_bits", self.state_bits) != self.state_bits for g in state_dict["param_groups"]):
+            raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
         for i, p in zip(saved, params):
-            for k, v in state_dict["state"].get(i, {}).items():
-                if torch.is_tensor(v):
-                    self.state[p][k] = v.detach().to(device=p.device, copy=True).contiguous()
-                else:
-                    self.state[p][k] = v
+            st = state_dict["state"].get(i)
+            if st and set(st) != {"step", *self._layout(p)}:
+                raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
+            for k, (shape, dtype) in self._layout(p).items() if st else ():
+                if tuple(st[k].shape) != tuple(shape) or st[k].dtype != dtype:
+                    raise ValueError(f"AdamW: saved {k} is {st[k].dtype} {tuple(st[k].shape)}, not {dtype} {tuple(shape)}")
+        super().load_state_dict(state_dict)
+        for i, p in zip(saved, params):
+            if state_dict["state"].get(i):
+                self.state[p] = {k: v.detach().to(device=p.device, copy=True).contiguous() if torch.is_tensor(v) else int(v)
+                                 for k, v in state_dict["state"][i].items()}
 
 
 def _check_param(p):

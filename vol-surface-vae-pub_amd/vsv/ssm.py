@@ -217,7 +217,9 @@ def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=Tru
     state is to decay), b, c (B, T, [G,] N), skip, dt_bias (D).  softplus=False takes dt + dt_bias as the time step itself.
     initial_state (B, D, N).  Returns y (B, T, D) [, the state behind the last step (B, D, N) in float32].
 
-    For gradients the states before every eighth step are kept (2 N bytes per element of x, in float32)."""
+    For gradients the states before every eighth step are kept (in float32: N / 2 bytes per element of x, N rounded up to
+    4, 8 or 16).  A training step captured into a HIP graph wants parameters without a live eager graph of their own, as any
+    captured backward pass of torch's does."""
     what = "ssm_scan"
     if not isinstance(x, _Tensor) or x.dim() != 3:
         raise ValueError(f"{what}: x must be a tensor (B, T, D)")
@@ -298,6 +300,8 @@ class SsmMemory(torch.nn.Module):
 
     def __init__(self, input_size, hidden_size, state_size=16, taps=4, dt_rank=None):
         super().__init__()
+        if not 1 <= state_size <= _lib.VSV_SSM_MAX_STATE or not 1 <= taps <= _lib.VSV_CONV_MAX_TAPS:
+            raise ValueError(f"SsmMemory: 1 to {_lib.VSV_SSM_MAX_STATE} states and 1 to {_lib.VSV_CONV_MAX_TAPS} taps are built")
         self.hidden_size, self.state_size, self.taps = hidden_size, state_size, taps
         self.dt_rank = dt_rank or max(1, -(-hidden_size // 16))
         self.in_proj = torch.nn.Linear(input_size, 2 * hidden_size)
