@@ -271,13 +271,15 @@ constexpr int kTile = 8;             // steps per tile; training keeps the state
 struct ScanPlan {
     long seg;                        // steps per segment, a multiple of kTile
     int S;                           // segments
+    int P;                           // lanes that share a channel's states (forward; then S = 1)
 };
 
 struct ScanPos {
     long b, g, base, t0, t1, tz;     // sequence, group, first channel; the segment's steps [t0, t1), padding [t1, tz)
     int s;
     unsigned lane;                   // channel base + lane
-    bool live;
+    int part;                        // which R / P of its states this lane owns
+    bool live, writes;               // a channel of its own; and the one of its lanes that stores the channel's outputs
 };
 
 __device__ inline long seq_len_s(const int* lengths, long b, long T) {
@@ -286,8 +288,9 @@ __device__ inline long seq_len_s(const int* lengths, long b, long T) {
     return n < 0 ? 0 : n > T ? T : n;
 }
 
-__device__ inline ScanPos scan_pos(const vsv_ssm_desc& a, const ScanPlan& pl, unsigned blk, int s0) {
-    const unsigned Dg = (unsigned)(a.D / a.G), cb = (Dg + 63) / 64;
+template <int P = 1> __device__ inline ScanPos scan_pos(const vsv_ssm_desc& a, const ScanPlan& pl, unsigned blk, int s0) {
+    constexpr unsigned kCh = 64 / P;
+    const unsigned Dg = (unsigned)(a.D / a.G), cb = (Dg + kCh - 1) / kCh, ch = threadIdx.x % kCh;
     const unsigned w = (unsigned)(a.B * a.G) * cb;
     ScanPos p;
     p.s = (int)(blk / w) + s0;
@@ -295,10 +298,12 @@ __device__ inline ScanPos scan_pos(const vsv_ssm_desc& a, const ScanPlan& pl, un
     const unsigned c = blk % cb, bg = blk / cb;
     p.g = bg % (unsigned)a.G;
     p.b = bg / (unsigned)a.G;
-    p.base = p.g * Dg + c * 64;
-    const unsigned left = Dg - c * 64;
-    p.live = threadIdx.x < left;
-    p.lane = p.live ? threadIdx.x : left - 1;
+    p.base = p.g * Dg + c * kCh;
+    const unsigned left = Dg - c * kCh;
+    p.part = threadIdx.x / kCh;
+    p.live = ch < left;
+    p.writes = p.live && p.part == 0;
+    p.lane = p.live ? ch : left - 1;
     const long len = seq_len_s(a.lengths, p.b, a.T);
     p.t0 = p.s * pl.seg;
     p.tz = p.t0 + pl.seg < a.T ? p.t0 + pl.seg : a.T;
@@ -397,7 +402,7 @@ template <typename T> __device__ inline void tile_values(const T (&r)[kTile], in
 // (a dead lane's offset lies behind the buffer's end, where stores are dropped)
 template <typename T> __device__ inline void tile_store(T* row, long D, const ScanPos& p, int left, const float (&v)[kTile]) {
     const auto r = __builtin_amdgcn_make_buffer_rsrc(row, 0, 0x7fffffff, 0x00020000);
-    const int voff = p.live ? (int)(p.lane * (unsigned)sizeof(T)) : (int)0xfffffff0;
+    const int voff = p.writes ? (int)(p.lane * (unsigned)sizeof(T)) : (int)0xfffffff0;
     const int step = (int)(D * (long)sizeof(T));
 #pragma unroll
     for (int i = 0; i < kTile; ++i) {
@@ -436,9 +441,25 @@ template <int R> __device__ inline void store_states(float* p, long D, long d, c
 
 __device__ inline int tile_left(const ScanPos& p, long t) { return p.t1 - t < kTile ? (int)(p.t1 - t) : kTile; }
 
-template <int R> __device__ inline void load_decay(const vsv_ssm_desc& a, long d, float (&A2)[R]) {
+template <int R> __device__ inline void load_decay(const vsv_ssm_desc& a, long d, float (&A2)[R], int n0 = 0) {
 #pragma unroll
-    for (int n = 0; n < R; ++n) A2[n] = n < a.N ? a.a[d * a.N + n] * kLog2e : 0.0f;
+    for (int n = 0; n < R; ++n) A2[n] = n0 + n < a.N ? a.a[d * a.N + n0 + n] * kLog2e : 0.0f;
+}
+
+// The sum over a channel's P lanes, which are 64 / P apart.
+template <int P> __device__ inline float part_sum(float v) {
+    static_assert(P == 1 || P == 2 || P == 4, "");
+    if constexpr (P >= 2) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        const unsigned r0 = r[0], r1 = r[1];
+        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+    }
+    if constexpr (P == 4) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        const unsigned r0 = r[0], r1 = r[1];
+        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+    }
+    return v;
 }
 
 // v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to
@@ -502,13 +523,15 @@ __global__ void __launch_bounds__(64) ssm_ends_kernel(const vsv_ssm_desc a, cons
     sd[(p.b * pl.S + p.s) * D + d] = sum;
 }
 
-template <typename T, int R>
+// P > 1: a channel's states are shared by P lanes, R / P each, and one pass runs over all of time.
+template <typename T, int R, int P>
 __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, const ScanPlan pl, const float* __restrict__ E,
                                                       const float* __restrict__ sd) {
     __shared__ alignas(16) float lds[2][kTile * 2 * R];
-    const ScanPos p = scan_pos(a, pl, blockIdx.x, 0);
+    constexpr int L = R / P;
+    const ScanPos p = scan_pos<P>(a, pl, blockIdx.x, 0);
     const long D = a.D, d = p.base + p.lane;
-    const int N = a.N;
+    const int N = a.N, n0 = p.part * L;
     T* y = (T*)a.y + p.b * a.T * D + p.base;
     const T *x = (const T*)a.x + p.b * a.x_bs + p.base + p.t0 * a.x_ts, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + p.t0 * a.dt_ts;
     const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base + p.t0 * a.gate_ts : nullptr;
@@ -521,12 +544,12 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
         if (gate) load_tile(gate, (int)(a.gate_ts * (long)sizeof(T)), p.lane, left, gr);
     };
     if (p.t0 < p.t1) fetch(tile_left(p, p.t0));
-    float A2[R], h[R];
-    load_decay<R>(a, d, A2);
+    float A2[L], h[L];
+    load_decay<L>(a, d, A2, n0);
 #pragma unroll
-    for (int n = 0; n < R; ++n) h[n] = n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n] : 0.0f;
-    fold_segments<R>(E, sd, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
-    const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
+    for (int n = 0; n < L; ++n) h[n] = n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
+    if constexpr (P == 1) fold_segments<R>(E, sd, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
+    const float skip = a.skip && p.part == 0 ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     float* saved = a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D : nullptr;
     int buf = 0;
     for (long t = p.t0; t < p.t1; t += kTile, buf ^= 1) {
@@ -545,25 +568,25 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
             fetch(tile_left(p, t + kTile));
         }
         if (saved) {
-            if (p.live) store_states<R>(saved, D, d, h);
+            if (p.live) store_states<L>(saved + n0 * D, D, d, h);
             saved += R * D;
         }
         order();
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            float b[R], c[R], e[R], acc[2] = {skip * xv[i], 0.0f};
-            bc_row<R>(lds[buf] + i * 2 * R, b);
-            bc_row<R>(lds[buf] + i * 2 * R + R, c);
+            float b[L], c[L], e[L], acc[2] = {skip * xv[i], 0.0f};
+            bc_row<L>(lds[buf] + i * 2 * R + n0, b);
+            bc_row<L>(lds[buf] + i * 2 * R + R + n0, c);
             const float dx = de[i] * xv[i];
-            decays<R>(de[i], A2, e);
-            order();
+            decays<L>(de[i], A2, e);
+            if constexpr (P == 1) order();
 #pragma unroll
-            for (int n = 0; n < R; ++n) {
+            for (int n = 0; n < L; ++n) {
                 h[n] = __builtin_fmaf(e[n], h[n], dx * b[n]);
                 acc[n & 1] = __builtin_fmaf(c[n], h[n], acc[n & 1]);
             }
-            yv[i] = acc[0] + acc[1];
-            order();
+            yv[i] = part_sum<P>(acc[0] + acc[1]);
+            if constexpr (P == 1) order();                               // (few states: steps side by side fit the registers)
         }
         if (gate) {
 #pragma unroll
@@ -571,12 +594,12 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
         }
         tile_store(y + t * D, D, p, left, yv);
     }
-    if (!p.live) return;
-    for (long t = p.t0 > p.t1 ? p.t0 : p.t1; t < p.tz; ++t) (y + t * D)[p.lane] = from_f<T>(0.0f);
-    if (a.state_out && p.s == pl.S - 1)
+    if (p.writes)
+        for (long t = p.t0 > p.t1 ? p.t0 : p.t1; t < p.tz; ++t) (y + t * D)[p.lane] = from_f<T>(0.0f);
+    if (a.state_out && p.live && p.s == pl.S - 1)
 #pragma unroll
-        for (int n = 0; n < R; ++n)
-            if (n < N) a.state_out[(p.b * D + d) * N + n] = h[n];
+        for (int n = 0; n < L; ++n)
+            if (n0 + n < N) a.state_out[(p.b * D + d) * N + n0 + n] = h[n];
 }
 
 // Backwards: g = dy silu(gate), q_t = c_t g_t + exp(delta_{t+1} a) q_{t+1} is the gradient of h_t.
@@ -984,19 +1007,24 @@ template <typename F> int by_states(int N, F&& f) {
 
 long ssm_blocks(const vsv_ssm_desc* a) { return (a->D / a->G + 63) / 64; }
 
-// The scan's split of time.  A split costs a second pass (1.8 times the work) and a launch, so it pays below half a wave per
-// SIMD (1024 of them) and from kSplitFrom steps on: then as many segments as make two waves per SIMD, none shorter than two
-// tiles, at most kMaxSegments (the start of a segment walks over those in front of it).
-constexpr long kMaxSegments = 64, kSplitFrom = 64, kSplitWaves = 2048;
+// How the work is divided.  A split of time costs a second pass (1.8 times the work) and a launch, so it pays below about half
+// a wave per SIMD (1024 of them): then as many segments as make two waves per SIMD, none shorter than two tiles, at most
+// kMaxSegments (the start of a segment walks over those in front of it).  Short sequences of so few waves are read forward in
+// one pass instead, with a channel's states shared by R / 4 lanes (64x60x100 float32: 26 us with one lane a channel).
+constexpr long kMaxSegments = 64, kSplitFrom = 64, kShareBelow = 192, kSplitWaves = 2048;
 
-ScanPlan scan_plan(const vsv_ssm_desc* a) {
+ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
     ScanPlan pl = {};
     const long waves = a->B * a->G * ssm_blocks(a), tiles = (a->T + kTile - 1) / kTile;
     long S = 1;
-    if (waves > 0 && waves < 512 && a->T >= kSplitFrom) {
-        S = (kSplitWaves + waves - 1) / waves;
-        if (S > tiles / 2) S = tiles / 2;
-        if (S > kMaxSegments) S = kMaxSegments;
+    pl.P = 1;
+    if (waves > 0 && waves < 512) {
+        if (forward && a->T < kShareBelow) pl.P = padded_states(a->N) / 4;
+        else if (a->T >= kSplitFrom) {
+            S = (kSplitWaves + waves - 1) / waves;
+            if (S > tiles / 2) S = tiles / 2;
+            if (S > kMaxSegments) S = kMaxSegments;
+        }
     }
     const long per = tiles > 0 ? (tiles + S - 1) / S : 1;
     pl.seg = per * kTile;
@@ -1083,7 +1111,7 @@ extern "C" size_t vsv_ssm_saved_floats(const vsv_ssm_desc* a) {
 
 extern "C" size_t vsv_ssm_scan_ws_bytes(const vsv_ssm_desc* a) {
     if (check_ssm(a, "vsv_ssm_scan_ws_bytes")) return 0;
-    return ends_floats(a, scan_plan(a)) * sizeof(float);
+    return ends_floats(a, scan_plan(a, true)) * sizeof(float);
 }
 
 extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, void* stream) {
@@ -1092,7 +1120,7 @@ extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, vo
     const size_t need = vsv_ssm_scan_ws_bytes(a);
     if (ws_bytes < need || (need && !aligned(ws, 16)) || (need && !ws)) { set_error("vsv_ssm_scan: workspace too small or not on 16 bytes"); return -1; }
     if (a->saved && !aligned(a->saved, 16)) { set_error("vsv_ssm_scan: saved must be on 16 bytes"); return -1; }
-    const ScanPlan pl = scan_plan(a);
+    const ScanPlan pl = scan_plan(a, true);
     const long waves = a->B * a->G * ssm_blocks(a);
     if (waves > kMaxBlocks / pl.S) { set_error("vsv_ssm_scan: too many sequences and channels for one call"); return -2; }
     float *E = (float*)ws, *sd = E + (size_t)a->B * pl.S * padded_states(a->N) * a->D;
@@ -1103,7 +1131,11 @@ extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, vo
             hipLaunchKernelGGL((ssm_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
             if (int rc = op_launch_check("ssm_ends_kernel")) return rc;
         }
-        hipLaunchKernelGGL((ssm_scan_kernel<T, R>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+        if (R > 4 && pl.P > 1) {
+            constexpr int P = R / 4, kCh = 64 / P;
+            const long groups = a->B * a->G * ((a->D / a->G + kCh - 1) / kCh);
+            hipLaunchKernelGGL((ssm_scan_kernel<T, R, P>), dim3((unsigned)groups), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+        } else hipLaunchKernelGGL((ssm_scan_kernel<T, R, 1>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
         return op_launch_check("ssm_scan_kernel");
     }); });
 }
@@ -1114,7 +1146,7 @@ size_t part_bc_floats(const vsv_ssm_desc* a) { return (size_t)ssm_blocks(a) * a-
 
 extern "C" size_t vsv_ssm_scan_backward_ws_bytes(const vsv_ssm_desc* a) {
     if (check_ssm(a, "vsv_ssm_scan_backward_ws_bytes")) return 0;
-    const ScanPlan pl = scan_plan(a);
+    const ScanPlan pl = scan_plan(a, false);
     return (round4(ends_floats(a, pl)) + round4(part_bc_floats(a)) +
             (size_t)a->B * pl.S * (padded_states(a->N) + 2) * a->D) * sizeof(float);
 }
@@ -1129,7 +1161,7 @@ extern "C" int vsv_ssm_scan_backward(const vsv_ssm_desc* a, const vsv_ssm_grads*
         set_error("vsv_ssm_scan_backward: workspace too small or not on 16 bytes"); return -1;
     }
     if (a->saved && !aligned(a->saved, 16)) { set_error("vsv_ssm_scan_backward: saved must be on 16 bytes"); return -1; }
-    const ScanPlan pl = scan_plan(a);
+    const ScanPlan pl = scan_plan(a, false);
     const int R0 = padded_states(a->N);
     const long nb = ssm_blocks(a), waves = a->B * a->G * nb, rows = a->B * a->T * a->G;
     if (waves > kMaxBlocks / pl.S) { set_error("vsv_ssm_scan_backward: too many elements for one call"); return -2; }
