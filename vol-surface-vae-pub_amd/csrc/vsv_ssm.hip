@@ -34,9 +34,7 @@ __device__ inline float conv_silu(float s) {
 // One read of x and one write of y (2K flops an element): bound by memory.  A thread owns VEC neighbouring channels and a
 // chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it works on kRows rows at a
 // time, with the next ones under way.
-constexpr int kRows = 4, kConvVec = 4;
-
-template <typename T, int K, int VEC> struct ConvRows {
+template <typename T, int K, int VEC, int kRows> struct ConvRows {
     const T* x;                      // the sequence's row 0, at this thread's channels
     const float* st;                 // state_in's, or null
     long ts, D, len;
@@ -60,14 +58,14 @@ template <typename T, int K, int VEC> struct ConvRows {
     }
 };
 
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, int kRows>
 __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_desc a, long chunk, long n_chunk, long n_vec) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
     if (id >= a.B * n_chunk * n_vec) return;
     const long dv = id % n_vec, bc = id / n_vec, ch = bc % n_chunk, b = bc / n_chunk;
     const long d0 = dv * VEC, t0 = ch * chunk, t1 = t0 + chunk < a.T ? t0 + chunk : a.T;
     T* y = (T*)a.y + b * a.T * a.D + d0;
-    ConvRows<T, K, VEC> in(a, b, d0);
+    ConvRows<T, K, VEC, kRows> in(a, b, d0);
     float w[VEC][K], bias[VEC], xs[K - 1 + kRows][VEC];
     if (t0 < in.len) in.fetch(t0);
 #pragma unroll
@@ -120,7 +118,7 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
 // ds = dy act'(pre) (pre computed again from x), dx[t] = sum_k w[k] ds[t+K-1-k], dw[k] = sum_t ds[t] xs[t-K+1+k],
 // dbias = sum_t ds.  The same chunks; a chunk reads K-1 rows beyond each end, its sums over time go to `part`
 // (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, int kRows>
 __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_conv_desc a, const vsv_short_conv_grads g, long chunk, long n_chunk,
                                                              long n_vec, float* __restrict__ part) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
@@ -130,7 +128,7 @@ __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_con
     const T* dy = (const T*)g.dy + b * g.dy_bs + d0;
     T* dx = (T*)g.dx + b * a.T * a.D + d0;
     const float* dso = g.d_state_out ? g.d_state_out + b * (K - 1) * a.D + d0 : nullptr;
-    ConvRows<T, K, VEC> in(a, b, d0);
+    ConvRows<T, K, VEC, kRows> in(a, b, d0);
     Pack<T, VEC> dyr[kRows];
     auto fetch = [&](long t) {
         in.fetch(t);
@@ -951,26 +949,36 @@ int check_conv(const vsv_short_conv_desc* a, const char* what) {
     return 0;
 }
 
-// Four channels per access where every row starts on such a word (eight in 16 bits need all registers in the backward pass and
-// gain nothing in the forward one).
-bool conv_wide(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, size_t size) {
-    constexpr long v = kConvVec;
+// Whether every row starts on a word of v elements.
+bool conv_words(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, size_t size, long v) {
     bool ok = a->D % v == 0 && a->x_bs % v == 0 && a->x_ts % v == 0 && aligned(a->x, v * size) && aligned(a->y, v * size);
     if (g) ok = ok && g->dy_bs % v == 0 && g->dy_ts % v == 0 && aligned(g->dy, v * size) && aligned(g->dx, v * size);
     return ok;
+}
+// Channels per thread: four where the rows allow it; backward eight in 16 bits (two rows under way instead of four fit the
+// registers: 8x2048x4096 bf16 108 us for 131; forward they are slower, 85 for 74).
+int conv_vec(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g) {
+    const size_t size = a->dtype == VSV_F32 ? 4 : 2;
+    if (g && size == 2 && conv_words(a, g, size, 8)) return 8;
+    return conv_words(a, g, size, 4) ? 4 : 1;
 }
 
 // Time steps per thread: the longer, the less is read twice and the fewer sums are left over, as long as the threads fill the
 // chip.  Forward eight waves for every SIMD (8x2048x4096 bf16: two 87, four 77, eight 74 us); backward, where a chunk leaves K + 1
 // sums per channel, two (131 us, four 138).
 constexpr long kConvFill = 524288, kConvBwdFill = 131072;
-long conv_chunk(const vsv_short_conv_desc* a, long fill) {
-    const long rows = a->B * (a->D / (a->D % kConvVec == 0 ? kConvVec : 1));
+long conv_chunk(const vsv_short_conv_desc* a, long fill, long vec) {
+    const long rows = a->B * (a->D / vec);
     long chunk = 16;
     while (chunk < 256 && rows * ((a->T + 2 * chunk - 1) / (2 * chunk)) >= fill) chunk *= 2;
     return chunk;
 }
-long conv_chunks(const vsv_short_conv_desc* a, long fill) { const long c = conv_chunk(a, fill); return a->T > 0 ? (a->T + c - 1) / c : 1; }
+long conv_chunks(const vsv_short_conv_desc* a, long chunk) { return a->T > 0 ? (a->T + chunk - 1) / chunk : 1; }
+// The backward pass's chunk goes by the sizes alone, so that its workspace does too.
+long conv_bwd_chunk(const vsv_short_conv_desc* a) {
+    const bool half = a->dtype != VSV_F32;
+    return conv_chunk(a, kConvBwdFill, half && a->D % 8 == 0 ? 8 : a->D % 4 == 0 ? 4 : 1);
+}
 
 template <typename F> int by_taps(int K, F&& f) {
     switch (K) {
@@ -1045,43 +1053,46 @@ using namespace vsv;
 extern "C" int vsv_short_conv(const vsv_short_conv_desc* a, void* stream) {
     if (int rc = check_conv(a, "vsv_short_conv")) return rc;
     if (a->B == 0) return 0;
-    return by_dtype(a->dtype, "vsv_short_conv", [&](auto t) {
+    const int vec = conv_vec(a, nullptr);
+    const long chunk = conv_chunk(a, kConvFill, vec), nc = conv_chunks(a, chunk), nv = a->D / vec, blocks = (a->B * nc * nv + 255) / 256;
+    if (blocks > kMaxBlocks) { set_error("vsv_short_conv: too many elements for one call"); return -2; }
+    return by_dtype(a->dtype, "vsv_short_conv", [&](auto t) { return by_taps(a->K, [&](auto k) {
         using T = decltype(t);
-        return by_taps(a->K, [&](auto k) {
-            constexpr int K = decltype(k)::value;
-            const bool wide = conv_wide(a, nullptr, sizeof(T));
-            const long nc = conv_chunks(a, kConvFill), nv = wide ? a->D / kConvVec : a->D, blocks = (a->B * nc * nv + 255) / 256;
-            if (blocks > kMaxBlocks) { set_error("vsv_short_conv: too many elements for one call"); return -2; }
-            if (wide) hipLaunchKernelGGL((short_conv_kernel<T, K, kConvVec>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a, kConvFill), nc, nv);
-            else hipLaunchKernelGGL((short_conv_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, conv_chunk(a, kConvFill), nc, nv);
-            return op_launch_check("short_conv_kernel");
-        });
-    });
+        constexpr int K = decltype(k)::value;
+        if (vec == 4) hipLaunchKernelGGL((short_conv_kernel<T, K, 4, 4>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, chunk, nc, nv);
+        else hipLaunchKernelGGL((short_conv_kernel<T, K, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, chunk, nc, nv);
+        return op_launch_check("short_conv_kernel");
+    }); });
 }
 
 extern "C" size_t vsv_short_conv_backward_ws_bytes(const vsv_short_conv_desc* a) {
     if (check_conv(a, "vsv_short_conv_backward_ws_bytes")) return 0;
-    return (size_t)a->B * conv_chunks(a, kConvBwdFill) * (a->K + 1) * a->D * sizeof(float);
+    return (size_t)a->B * conv_chunks(a, conv_bwd_chunk(a)) * (a->K + 1) * a->D * sizeof(float);
 }
 
 extern "C" int vsv_short_conv_backward(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = check_conv(a, "vsv_short_conv_backward")) return rc;
     if (!g || (a->B > 0 && a->T > 0 && (!g->dy || !g->dx))) { set_error("vsv_short_conv_backward: null pointer"); return -1; }
-    if (ws_bytes < vsv_short_conv_backward_ws_bytes(a) || (!ws && a->B > 0)) { set_error("vsv_short_conv_backward: workspace too small"); return -1; }
-    const long nc = conv_chunks(a, kConvBwdFill), M = (a->K + 1) * a->D;
+    if (ws_bytes < vsv_short_conv_backward_ws_bytes(a) || (a->B > 0 && (!ws || !aligned(ws, 16)))) {
+        set_error("vsv_short_conv_backward: workspace too small or not on 16 bytes"); return -1;
+    }
+    const int vec = conv_vec(a, g);
+    const long chunk = conv_bwd_chunk(a), nc = conv_chunks(a, chunk), nv = a->D / vec, M = (a->K + 1) * a->D, blocks = (a->B * nc * nv + 255) / 256;
+    if (blocks > kMaxBlocks) { set_error("vsv_short_conv_backward: too many elements for one call"); return -2; }
     if (a->B > 0) {
-        const int rc = by_dtype(a->dtype, "vsv_short_conv_backward", [&](auto t) {
+        const int rc = by_dtype(a->dtype, "vsv_short_conv_backward", [&](auto t) { return by_taps(a->K, [&](auto k) {
             using T = decltype(t);
-            return by_taps(a->K, [&](auto k) {
-                constexpr int K = decltype(k)::value;
-                const bool wide = conv_wide(a, g, sizeof(T));
-                const long nv = wide ? a->D / kConvVec : a->D, blocks = (a->B * nc * nv + 255) / 256;
-                if (blocks > kMaxBlocks) { set_error("vsv_short_conv_backward: too many elements for one call"); return -2; }
-                if (wide) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, kConvVec>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a, kConvBwdFill), nc, nv, (float*)ws);
-                else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, conv_chunk(a, kConvBwdFill), nc, nv, (float*)ws);
-                return op_launch_check("short_conv_bwd_kernel");
-            });
-        });
+            constexpr int K = decltype(k)::value;
+            if constexpr (sizeof(T) == 2) {
+                if (vec == 8) {
+                    hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 8, 2>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, chunk, nc, nv, (float*)ws);
+                    return op_launch_check("short_conv_bwd_kernel");
+                }
+            }
+            if (vec == 4) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 4, 4>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, chunk, nc, nv, (float*)ws);
+            else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, chunk, nc, nv, (float*)ws);
+            return op_launch_check("short_conv_bwd_kernel");
+        }); });
         if (rc) return rc;
     }
     hipLaunchKernelGGL(sum_conv_parts_kernel, dim3((unsigned)((M + 63) / 64)), dim3(256), 0, (hipStream_t)stream, (const float*)ws, a->B * nc, a->D, a->K, g->dw, g->dbias);
