@@ -7,12 +7,10 @@ parameter groups, state_dict, and the model classes' train_step(x, optimizer).
 """
 from __future__ import annotations
 
-import array
-
 import torch
 
 from . import lib as _lib
-from .ssm import _TYPES, _call, _touched
+from . import native as _native
 
 
 class AdamW(torch.optim.Optimizer):
@@ -67,37 +65,28 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        state, calls = self.state, []
-        for group in self.param_groups:                                    # everything is checked before anything is launched
+        state, calls, states = self.state, [], []
+        wide = self.state_bits == 32
+        for group in self.param_groups:
             rows = {}
             for p in group["params"]:
                 g = p.grad
-                if g is None:
-                    continue
-                if p.dtype not in _TYPES or not p.is_contiguous():
-                    _check_param(p)
-                if g.layout is not torch.strided or g.dtype is not p.dtype or g.get_device() != p.get_device() or g.shape != p.shape:
-                    raise ValueError("AdamW: a gradient needs its parameter's type, device and shape, and no sparse layout")
-                if not p.is_cuda:
-                    raise RuntimeError("AdamW: parameters must be on a GPU; there is no CPU fallback")
-                st = state[p] or self._init_state(p)
-                m = st["exp_avg"]
-                if m.shape != p.shape or m.get_device() != p.get_device():
-                    raise ValueError("AdamW: a parameter has changed its shape or device since its state was made")
-                rows.setdefault((p.dtype, p.get_device(), st["step"]), []).append((p, g if g.is_contiguous() else g.contiguous(), st))
-            calls += [(group, *key, rows[key]) for key in rows]
-        if calls and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
-        for group, dtype, at, step, rows in calls:
-            table = _table(rows, self.state_bits)
+                if g is not None:
+                    st = state[p] or self._init_state(p)
+                    rows.setdefault(st["step"], []).append((p, g, st))
             b1, b2 = group["betas"]
-            _call("vsv_adamw_multi", at, table.buffer_info()[0], len(rows), _TYPES[dtype], self.state_bits, float(group["lr"]),
-                  float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step + 1)
-            written = []
-            for p, _, st in rows:
-                st["step"] = step + 1
-                written += (p, st["exp_avg"], st["exp_avg_sq"])
-            _touched(written)
+            for step, part in rows.items():
+                ps, gs, sts = zip(*part)
+                calls.append((ps, gs, [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts],
+                              [] if wide else [st["exp_avg_scale"] for st in sts], [] if wide else [st["exp_avg_sq_scale"] for st in sts],
+                              float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step + 1))
+                states += sts
+        if calls:
+            if calls[0][0][0].is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
+            _native.load().adamw_step(self.state_bits, calls)              # (checks everything before it launches anything)
+            for st in states:
+                st["step"] += 1
         return loss
 
     @torch.no_grad()
@@ -105,17 +94,10 @@ class AdamW(torch.optim.Optimizer):
         """([exp_avg], [exp_avg_sq]) in float32 of the parameters that have been stepped, in the groups' order: the state's own
         tensors with 32 bits, the values that the codes stand for with 8."""
         states = [st for st in (self.state.get(p) for g in self.param_groups for p in g["params"]) if st]
+        m, v = [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
         if self.state_bits == 32:
-            return [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
-        ms = [torch.empty_like(st["exp_avg"], dtype=torch.float32) for st in states]
-        vs = [torch.empty_like(m) for m in ms]
-        rows = {}
-        for m, v, st in zip(ms, vs, states):
-            rows.setdefault(m.get_device(), []).append((m, v, st))
-        for at, part in rows.items():
-            table = _table(part, 8)
-            _call("vsv_adamw_read8", at, table.buffer_info()[0], len(part))
-        return ms, vs
+            return m, v
+        return _native.load().adamw_read8(m, v, [st["exp_avg_scale"] for st in states], [st["exp_avg_sq_scale"] for st in states])
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments keep their own types (torch's casts floating state to the parameter's), and nothing that
@@ -139,20 +121,7 @@ class AdamW(torch.optim.Optimizer):
 
 
 def _check_param(p):
-    if p.dtype not in _TYPES:
+    if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError(f"AdamW: parameters must be float32, bfloat16 or float16, not {p.dtype}")
     if not p.is_contiguous():
         raise ValueError("AdamW: parameters must be contiguous")
-
-
-def _table(rows, bits):
-    """struct vsv_adamw_tensor[len(rows)] of (p, g, state) rows, as 64-bit words."""
-    words = []
-    for p, g, st in rows:
-        m = st["exp_avg"]
-        if bits == 8:
-            words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
-                      st["exp_avg_sq_scale"].data_ptr(), m.numel())
-        else:
-            words += (p.data_ptr(), g.data_ptr(), m.data_ptr(), st["exp_avg_sq"].data_ptr(), 0, 0, m.numel())
-    return array.array("Q", words)

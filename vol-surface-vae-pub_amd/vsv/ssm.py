@@ -17,198 +17,39 @@ and gradients zero there, states taken at the length; a length outside [0, T] co
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 
 import torch
 
 from . import lib as _lib
-
-_GPU = "there is no CPU fallback"
-
-
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}              # VSV_F32, VSV_BF16, VSV_F16
-_Tensor, _f32_type = torch.Tensor, torch.float32
-_entries = {}
+from . import native as _native
 
 
-def _last(t):
-    """t itself where its last dimension is contiguous, else a copy."""
-    return t if t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+def _call(name, named, *args):
+    """An entry of the native side.  What its signature cannot take is not a tensor where one is wanted: named says which."""
+    try:
+        return getattr(_native.load(), name)(*args)
+    except TypeError:
+        for k, t in named.items():
+            if not isinstance(t, torch.Tensor) and not (t is None and k not in ("x", "weight", "dt", "a", "b", "c", "state")):
+                raise ValueError(f"{name}: {k} must be a tensor, not {t!r}") from None
+        raise
 
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _seq(what, name, t, shape, dtype=None):
-    if not isinstance(t, _Tensor) or t.shape != shape:
-        raise ValueError(f"{what}: {name} must be a tensor of shape {tuple(shape)}, not {tuple(t.shape) if isinstance(t, _Tensor) else t!r}")
-    if t.dtype not in _TYPES or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{what}: {name} must be {dtype or 'float32, bfloat16 or float16'}, not {t.dtype}")
-    return t if t.is_contiguous() else _last(t)
-
-
-def _f32(what, name, t, shape):
-    if t is None:
-        return None
-    if not isinstance(t, _Tensor) or t.shape != shape or t.dtype is not _f32_type:
-        raise ValueError(f"{what}: {name} must be a float32 tensor of shape {tuple(shape)}"
-                         + (f", not {t.dtype} {tuple(t.shape)}" if isinstance(t, _Tensor) else f", not {t!r}"))
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _lengths(what, t, B):
-    if t is None:
-        return None
-    if not isinstance(t, _Tensor) or t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: lengths must be an int32 or int64 tensor of shape ({B},)")
-    if t.dtype == torch.int64:
-        t = t.clamp(0, 2**31 - 1).to(torch.int32)
-    return t.contiguous()
-
-
-def _same_gpu(what, x, *others):
-    if not x.is_cuda:
-        raise RuntimeError(f"{what}: tensors must be on a GPU; {_GPU}")
-    at = x.get_device()
-    for t in others:
-        if t is not None and t.get_device() != at:
-            raise ValueError(f"{what}: tensors are on {t.device} and {x.device}")
-
-
-def _call(name, at, *args):
-    """One entry point on the current stream of GPU `at`."""
-    fn = _entries.get(name)
-    if fn is None:
-        fn = _entries[name] = getattr(_lib.load(), name)
-    if torch._C._cuda_getDevice() == at:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
-    else:
-        with torch.cuda.device(at):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
-    if rc:
-        _lib.check(rc, name)
-
-
-def _size(name, desc):
-    """A size that the library answers for a descriptor."""
-    fn = _entries.get(name)
-    if fn is None:
-        fn = _entries[name] = getattr(_lib.load(), name)
-    return fn(desc)
-
-
-def _workspace(nbytes, device):
-    return torch.empty(nbytes or 16, dtype=torch.uint8, device=device)
-
-
-def _wants_grad(*ts):
-    if not torch.is_grad_enabled():
-        return False
-    for t in ts:
-        if t is not None and t.requires_grad:
-            return True
-    return False
-
-
-def _touched(t):
-    """What an in-place operation leaves on a tensor that was written through its address."""
-    torch.autograd.graph.increment_version(t)
-
-
-# ---- short causal convolution ------------------------------------------------------------------------------------
 
 def short_conv(x, weight, bias=None, *, silu=True, initial_state=None, lengths=None, return_state=False):
     """y[:, t] = act(bias + sum_k weight[:, k] x[:, t - K + 1 + k]) per channel, act = silu or (silu=False) nothing.
 
     x (B, T, D), weight (D, K) with 1 to 4 taps, bias (D).  initial_state (B, K - 1, D): the inputs before the first (zeros
     without it).  Returns y (B, T, D) [, the last K - 1 inputs (B, K - 1, D) in float32]."""
-    what = "short_conv"
-    if not isinstance(x, _Tensor) or x.dim() != 3:
-        raise ValueError(f"{what}: x must be a tensor (B, T, D)")
-    B, T, D = x.shape
-    if not isinstance(weight, _Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= _lib.VSV_CONV_MAX_TAPS or D < 1:
-        raise ValueError(f"{what}: weight must be a tensor (D, K) with 1 to {_lib.VSV_CONV_MAX_TAPS} taps")
-    K = weight.shape[1]
-    x = _seq(what, "x", x, (B, T, D))
-    weight, bias = _f32(what, "weight", weight, (D, K)), _f32(what, "bias", bias, (D,))
-    initial_state = _f32(what, "initial_state", initial_state, (B, K - 1, D))
-    lengths = _lengths(what, lengths, B)
-    _same_gpu(what, x, weight, bias, initial_state, lengths)
-    if _wants_grad(x, weight, bias, initial_state):
-        from .autograd import ShortConv
-        y, state = ShortConv.apply(x, weight, bias, initial_state, lengths, bool(silu), bool(return_state))
-    else:
-        y, state, _ = conv_forward(x, weight, bias, initial_state, lengths, silu, return_state)
-    return (y, state) if return_state else y
-
-
-def conv_forward(x, weight, bias, state_in, lengths, silu, want_state):
-    """The launch behind short_conv: (y, state | None, the descriptor vsv_short_conv_backward takes again)."""
-    (B, T, D), K = x.shape, weight.shape[1]
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    state = torch.empty((B, K - 1, D), dtype=torch.float32, device=x.device) if want_state else None
-    d = _lib.VsvShortConv(_TYPES[x.dtype], K, int(silu), B, T, D, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(),
-                          _ptr(bias), _ptr(state_in), _ptr(lengths), y.data_ptr(), _ptr(state) or None)
-    _call("vsv_short_conv", x.get_device(), C.byref(d))
-    return y, state, d
+    out = _call("short_conv", dict(x=x, weight=weight, bias=bias, initial_state=initial_state, lengths=lengths), x, weight, bias, silu,
+                initial_state, lengths, return_state)
+    return (out[0], out[1]) if return_state else out[0]
 
 
 def short_conv_step(x, state, weight, bias=None, *, silu=True):
     """short_conv for one new token of every row: x (B, D) -> y (B, D); state (B, K - 1, D), contiguous float32, is updated in
-    place.  No gradients."""
-    what = "short_conv_step"
-    if not isinstance(x, _Tensor) or x.dim() != 2:
-        raise ValueError(f"{what}: x must be a tensor (B, D)")
-    B, D = x.shape
-    if not isinstance(weight, _Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= _lib.VSV_CONV_MAX_TAPS or D < 1:
-        raise ValueError(f"{what}: weight must be a tensor (D, K) with 1 to {_lib.VSV_CONV_MAX_TAPS} taps")
-    K = weight.shape[1]
-    x = _seq(what, "x", x, (B, D))
-    weight, bias = _f32(what, "weight", weight, (D, K)), _f32(what, "bias", bias, (D,))
-    _in_place(what, state, (B, K - 1, D))
-    _same_gpu(what, x, weight, bias, state)
-    if _wants_grad(x, weight, bias, state):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    d = _lib.VsvShortConv(_TYPES[x.dtype], K, int(silu), B, 1, D, x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _ptr(bias),
-                          None, None, y.data_ptr(), state.data_ptr())
-    _call("vsv_short_conv_step", x.get_device(), C.byref(d))
-    _touched(state)
-    return y
-
-
-def _in_place(what, state, shape):
-    if not isinstance(state, _Tensor) or state.shape != shape or state.dtype != torch.float32 or not state.is_contiguous():
-        raise ValueError(f"{what}: state must be a contiguous float32 tensor of shape {tuple(shape)} (it is updated in place)")
-
-
-# ---- selective scan ----------------------------------------------------------------------------------------------
-
-def _grouped(what, name, t, lead, D, N, dtype):
-    """b or c with its group dimension."""
-    if isinstance(t, _Tensor) and t.dim() == len(lead) + 1:
-        t = t.unsqueeze(-2)
-    if not isinstance(t, _Tensor) or t.dim() != len(lead) + 2 or t.shape[-2] < 1 or D % t.shape[-2]:
-        raise ValueError(f"{what}: {name} must be a tensor ({', '.join(map(str, lead))}, [G,] N) with G a divisor of D = {D}")
-    return _seq(what, name, t, (*lead, t.shape[-2], N), dtype)
-
-
-def _scan_args(what, x, dt, a, b, c, skip, gate, dt_bias, lead):
-    """The checked operands; b and c with their group dimension."""
-    D = x.shape[-1]
-    if not isinstance(a, _Tensor) or a.dim() != 2 or a.shape[0] != D or not 1 <= a.shape[1] <= _lib.VSV_SSM_MAX_STATE or D < 1:
-        raise ValueError(f"{what}: a must be a tensor (D, N) with 1 to {_lib.VSV_SSM_MAX_STATE} states")
-    N = a.shape[1]
-    x = _seq(what, "x", x, (*lead, D))
-    dt = _seq(what, "dt", dt, (*lead, D), x.dtype)
-    gate = None if gate is None else _seq(what, "gate", gate, (*lead, D), x.dtype)
-    b, c = _grouped(what, "b", b, lead, D, N, x.dtype), _grouped(what, "c", c, lead, D, N, x.dtype)
-    if b.shape != c.shape:
-        raise ValueError(f"{what}: b has {b.shape[-2]} groups and c {c.shape[-2]}")
-    a, skip, dt_bias = _f32(what, "a", a, (D, N)), _f32(what, "skip", skip, (D,)), _f32(what, "dt_bias", dt_bias, (D,))
-    return x, dt, a, b, c, skip, gate, dt_bias
+    place.  No gradients.  Bit for bit what short_conv gives for the same inputs."""
+    return _call("short_conv_step", dict(x=x, state=state, weight=weight, bias=bias), x, state, weight, bias, silu)
 
 
 def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=True, initial_state=None, lengths=None,
@@ -220,75 +61,16 @@ def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=Tru
     For gradients the states before every eighth step are kept (in float32: N / 2 bytes per element of x, N rounded up to
     4, 8 or 16).  A training step captured into a HIP graph wants parameters without a live eager graph of their own, as any
     captured backward pass of torch's does."""
-    what = "ssm_scan"
-    if not isinstance(x, _Tensor) or x.dim() != 3:
-        raise ValueError(f"{what}: x must be a tensor (B, T, D)")
-    B, T, D = x.shape
-    x, dt, a, b, c, skip, gate, dt_bias = _scan_args(what, x, dt, a, b, c, skip, gate, dt_bias, (B, T))
-    initial_state = _f32(what, "initial_state", initial_state, (B, D, a.shape[1]))
-    lengths = _lengths(what, lengths, B)
-    _same_gpu(what, x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths)
-    if _wants_grad(x, dt, a, b, c, skip, gate, dt_bias, initial_state):
-        from .autograd import SsmScan
-        y, state = SsmScan.apply(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths, bool(softplus), bool(return_state))
-    else:
-        y, state, _, _ = scan_forward(x, dt, a, b, c, skip, gate, dt_bias, initial_state, lengths, bool(softplus), return_state, False)
-    return (y, state) if return_state else y
-
-
-def _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, state_in, lengths, softplus, B, T, y, state):
-    D, N = a.shape
-    if T is not None:
-        x_bs, x_ts, _ = x.stride()
-        dt_bs, dt_ts, _ = dt.stride()
-        g_bs, g_ts, _ = gate.stride() if gate is not None else (0, 0, 0)
-        b_bs, b_ts, b_gs, _ = b.stride()
-        c_bs, c_ts, c_gs, _ = c.stride()
-    else:                                                                  # (B, D) rows: one step, no time stride
-        T = 1
-        x_bs, x_ts, dt_bs, dt_ts, b_ts, c_ts, g_ts = x.stride(0), 0, dt.stride(0), 0, 0, 0, 0
-        g_bs = gate.stride(0) if gate is not None else 0
-        b_bs, b_gs, _ = b.stride()
-        c_bs, c_gs, _ = c.stride()
-    return _lib.VsvSsm(_TYPES[x.dtype], N, softplus, B, T, D, b.shape[-2], x.data_ptr(), x_bs, x_ts, dt.data_ptr(), dt_bs, dt_ts,
-                       _ptr(gate), g_bs, g_ts, b.data_ptr(), b_bs, b_ts, b_gs, c.data_ptr(), c_bs, c_ts, c_gs,
-                       a.data_ptr(), _ptr(skip), _ptr(dt_bias), _ptr(state_in), _ptr(lengths), y.data_ptr(), _ptr(state), None)
-
-
-def scan_forward(x, dt, a, b, c, skip, gate, dt_bias, state_in, lengths, softplus, want_state, save):
-    """The launches behind ssm_scan: (y, state | None, the descriptor vsv_ssm_scan_backward takes again, saved | None)."""
-    (B, T, D), N = x.shape, a.shape[1]
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    state = torch.empty((B, D, N), dtype=torch.float32, device=x.device) if want_state else None
-    d = _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, state_in, lengths, softplus, B, T, y, state)
-    ref = C.byref(d)
-    saved = None
-    if save:
-        saved = torch.empty(_size("vsv_ssm_saved_floats", ref), dtype=torch.float32, device=x.device)
-        d.saved = saved.data_ptr() or None
-    nbytes = _size("vsv_ssm_scan_ws_bytes", ref)
-    ws = _workspace(nbytes, x.device) if nbytes else None
-    _call("vsv_ssm_scan", x.get_device(), ref, _ptr(ws), nbytes)
-    return y, state, d, saved
+    out = _call("ssm_scan", dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, dt_bias=dt_bias, initial_state=initial_state, lengths=lengths),
+                x, dt, a, b, c, skip, gate, dt_bias, softplus, initial_state, lengths, return_state)
+    return (out[0], out[1]) if return_state else out[0]
 
 
 def ssm_step(x, dt, a, b, c, skip=None, gate=None, *, state, dt_bias=None, softplus=True):
     """ssm_scan for one new token of every row: x, dt [, gate] (B, D), b, c (B, [G,] N) -> y (B, D); state (B, D, N),
     contiguous float32, is updated in place.  No gradients."""
-    what = "ssm_step"
-    if not isinstance(x, _Tensor) or x.dim() != 2:
-        raise ValueError(f"{what}: x must be a tensor (B, D)")
-    B, D = x.shape
-    x, dt, a, b, c, skip, gate, dt_bias = _scan_args(what, x, dt, a, b, c, skip, gate, dt_bias, (B,))
-    _in_place(what, state, (B, D, a.shape[1]))
-    _same_gpu(what, x, dt, a, b, c, skip, gate, dt_bias, state)
-    if _wants_grad(x, dt, a, b, c, skip, gate, dt_bias, state):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    d = _scan_desc(x, dt, a, b, c, skip, gate, dt_bias, None, None, bool(softplus), B, None, y, state)
-    _call("vsv_ssm_step", x.get_device(), C.byref(d))
-    _touched(state)
-    return y
+    return _call("ssm_step", dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, state=state, dt_bias=dt_bias),
+                 x, dt, a, b, c, skip, gate, state, dt_bias, softplus)
 
 
 # ---- the memory they make up -------------------------------------------------------------------------------------
