@@ -299,6 +299,17 @@ def test_closure_scheduler_and_capture():
     assert opt.state[p]["step"] == 1
 
 
+def test_a_refused_step_changes_nothing():
+    from vsv.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(10, device="cuda")) for _ in range(2))
+    opt = AdamW([{"params": [p]}, {"params": [q], "lr": 0.5}])
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt.param_groups[1]["betas"] = (0.9, 1.0)
+    with pytest.raises(ValueError, match="hyper-parameters"):
+        opt.step()
+    assert opt.state[p]["step"] == 0 and torch.equal(p, torch.ones_like(p)) and not opt.state[p]["exp_avg"].any()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_model_train_step_takes_it(bits):
     """CVAEMemRand.train_step(x, optimizer) with this optimizer: the parameters after three steps against torch's own AdamW (32 bits:

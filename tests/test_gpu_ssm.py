@@ -470,3 +470,31 @@ def test_on_another_stream():
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+def test_views_with_their_sign_put_off():
+    from vsv.ssm import short_conv, ssm_scan
+    z = torch.randn(2, 20, 70, dtype=torch.complex64, device="cuda").conj()
+    w = torch.randn(70, 4, dtype=torch.complex64, device="cuda").conj()
+    assert z.imag.is_neg() and w.imag.is_neg()
+    assert torch.equal(short_conv(z.imag, w.imag), short_conv(z.imag.clone(), w.imag.clone()))
+    x, a, b = z.imag, -torch.rand(70, 8, device="cuda"), torch.randn(2, 20, 8, device="cuda")
+    assert torch.equal(ssm_scan(x, x, a, b, b, w.imag[:, 0], x), ssm_scan(x.clone(), x.clone(), a, b, b, w.imag[:, 0].clone(), x.clone()))
+
+
+def test_states_made_in_inference_mode():
+    from vsv.ssm import SsmMemory
+    mem = SsmMemory(6, 70).cuda()
+    x = torch.randn(3, 9, 6, device="cuda")
+    with torch.inference_mode():
+        whole, _ = mem(x)
+        _, state = mem(x[:, :8])
+        last = mem.step(x[:, 8], state)
+        # (three products of up to 70 terms one after the other, in float32, summed in another order: 3 * 70 * 2^-24 = 1.3e-5 of the
+        # terms' sizes, which are up to some times the sums')
+        assert (last - whole[:, 8]).abs().max() <= 1e-4 * whole.abs().max()
+    kept = [t.clone() for t in state]
+    with pytest.raises(RuntimeError, match="[Ii]nference"):                  # torch's own rule, and nothing has been written
+        mem.step(x[:, 8], state)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, k) for t, k in zip(state, kept))

@@ -136,6 +136,30 @@ def test_optimizer_refuses():
         AdamW([p], state_bits=8).load_state_dict({"state": {0: {"step": 1, "exp_avg": torch.zeros(4, 3)}}, "param_groups": opt.state_dict()["param_groups"]})
 
 
+def test_optimizer_refuses_parameters_that_share_memory():
+    from vsv.optim import AdamW
+    flat = torch.zeros(24)
+    p, q, r = (torch.nn.Parameter(flat[k:k + 8]) for k in (0, 8, 15))
+    with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="twice"):
+        AdamW([p, q, p])
+    for x in (p, q, r):
+        x.grad = torch.ones(8)
+    with pytest.raises(RuntimeError, match="GPU"):                          # side by side is fine
+        AdamW([p, q]).step()
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([p, q, r]).step()
+    tied = torch.nn.Parameter(torch.zeros(8))
+    opt = AdamW([{"params": [p]}, {"params": [tied]}])
+    tied.data, tied.grad = p.data, torch.ones(8)
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    opt = AdamW([{"params": [p]}, {"params": [q]}])
+    opt.param_groups[1]["lr"] = -1.0                                         # (a later group's, found before the first is stepped)
+    with pytest.raises(ValueError, match="hyper-parameters"):
+        opt.step()
+    assert opt.state[p]["step"] == 0
+
+
 def test_c_entries_check_their_arguments():
     from vsv import lib as vlib
     L = vlib.load()

@@ -314,10 +314,16 @@ template <int P = 1> __device__ inline ScanPos scan_pos(const vsv_ssm_desc& a, c
 __device__ inline void pin(float& v) { asm volatile("" : "+v"(v)); }
 __device__ inline void order() { __builtin_amdgcn_sched_barrier(0); }
 
+// Orders what the lanes of a wave store to shared memory and load from it (a workgroup is one wave; this is no instruction).
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // b and c of a tile: eight lanes to a step, four of them b's states and four c's, R / 4 each.  They are loaded a tile ahead,
 // whatever their strides, and laid down in the wave's own shared memory as float32, zeros behind the N states; a step then
 // reads its rows as broadcasts.  (Read through the scalar cache, with the next step's rows under way during the present
-// step, a wave alone on its SIMD took 1080 cycles a step: the scalar loads miss to L2, and only the latest can be waited for.)
+// step, 64x60x100 in float32 took 32 us for 26: the scalar loads miss to L2, and only the latest can be waited for.)
 template <typename T, int R> struct BcTile {
     static constexpr int V = R / 4;
     const T* at;                     // this lane's first state in the tile's first row of its own
@@ -346,7 +352,9 @@ template <typename T, int R> struct BcTile {
         float v[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] = to_f(raw[k]);
+        wave_fence();
         if (on) store_vec<float, V>(lds + to, v);
+        wave_fence();
     }
 };
 // H states of a row, the same for every lane
@@ -1182,7 +1190,7 @@ extern "C" int vsv_ssm_scan_backward(const vsv_ssm_desc* a, const vsv_ssm_grads*
         const int rc = by_dtype(a->dtype, "vsv_ssm_scan_backward", [&](auto t) { return by_states(a->N, [&](auto r) {
             using T = decltype(t);
             constexpr int R = decltype(r)::value;
-                if (pl.S > 1) {
+            if (pl.S > 1) {
                 hipLaunchKernelGGL((ssm_bwd_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd);
                 if (int rc = op_launch_check("ssm_bwd_ends_kernel")) return rc;
             }

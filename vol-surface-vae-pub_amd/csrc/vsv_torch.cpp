@@ -7,6 +7,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+
 #include "../../include/vsv_hip.h"
 
 namespace {
@@ -66,7 +68,8 @@ int type_code(const Tensor& t) {
     }
 }
 
-Tensor last_contiguous(const Tensor& t) {
+Tensor last_contiguous(const Tensor& t_) {
+    const Tensor t = t_.resolve_neg();                                     // (a conjugate's imaginary part is a view with its sign put off)
     if (t.is_contiguous()) return t;
     return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
@@ -82,7 +85,7 @@ Tensor f32(const char* what, const char* name, const OptTensor& t, at::IntArrayR
     if (!t || !t->defined()) return Tensor();
     TORCH_CHECK_VALUE(t->sizes() == shape && t->scalar_type() == at::kFloat && t->layout() == at::kStrided, what, ": ", name,
                       " must be a float32 tensor of shape ", shape, ", not ", t->scalar_type(), " ", t->sizes());
-    return t->contiguous();
+    return t->resolve_neg().contiguous();
 }
 
 Tensor int_lengths(const char* what, const OptTensor& t, int64_t B) {
@@ -94,7 +97,7 @@ Tensor int_lengths(const char* what, const OptTensor& t, int64_t B) {
 }
 
 void in_place(const char* what, const Tensor& t, at::IntArrayRef shape) {
-    TORCH_CHECK_VALUE(t.sizes() == shape && t.scalar_type() == at::kFloat && t.layout() == at::kStrided && t.is_contiguous(), what,
+    TORCH_CHECK_VALUE(t.sizes() == shape && t.scalar_type() == at::kFloat && t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg(), what,
                       ": state must be a contiguous float32 tensor of shape ", shape, " (it is updated in place)");
 }
 
@@ -225,8 +228,8 @@ Tensor short_conv_step(const Tensor& x_, const Tensor& state, const Tensor& weig
     c10::DeviceGuard guard(x.device());
     const Tensor y = whole_like(x);
     const auto d = conv_desc(x, w, bias, Tensor(), Tensor(), silu, y.data_ptr(), state);
+    state.unsafeGetTensorImpl()->bump_version();                           // (refuses an inference tensor outside inference mode)
     check(api.short_conv_step(&d, stream_of(x)), "vsv_short_conv_step");
-    state.unsafeGetTensorImpl()->bump_version();
     return y;
 }
 
@@ -362,8 +365,8 @@ Tensor ssm_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor
     c10::DeviceGuard guard(r.x.device());
     const Tensor y = whole_like(r.x);
     const auto d = scan_desc(r, Tensor(), Tensor(), softplus, y.data_ptr(), state);
-    check(api.ssm_step(&d, stream_of(r.x)), "vsv_ssm_step");
     state.unsafeGetTensorImpl()->bump_version();
+    check(api.ssm_step(&d, stream_of(r.x)), "vsv_ssm_step");
     return y;
 }
 
@@ -378,19 +381,38 @@ void state_fits(const Tensor& p, const Tensor& t, at::ScalarType type, int64_t n
                       "AdamW: a parameter has changed its shape or device since its state was made");
 }
 
+// One launch updates the tensors side by side, so none may hold another's elements.
+void apart(std::vector<std::pair<uintptr_t, uintptr_t>>& spans) {
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "AdamW: two parameters share memory");
+}
+
 void adamw_step(int bits, std::vector<AdamwCall> calls) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     for (auto& [p, g, m, v, ms, vs, lr, b1, b2, eps, wd, step] : calls) {   // everything is checked before anything is launched
+        TORCH_CHECK_VALUE(lr >= 0.0 && b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0 && wd >= 0.0, "AdamW: bad hyper-parameters lr=", lr,
+                          " betas=(", b1, ", ", b2, ") eps=", eps, " weight_decay=", wd);
         for (size_t i = 0; i < p.size(); ++i) {
             TORCH_CHECK_VALUE(type_code(p[i]) >= 0, "AdamW: parameters must be float32, bfloat16 or float16, not ", p[i].scalar_type());
             TORCH_CHECK_VALUE(p[i].is_contiguous(), "AdamW: parameters must be contiguous");
             TORCH_CHECK_VALUE(g[i].layout() == at::kStrided && g[i].scalar_type() == p[i].scalar_type() && g[i].device() == p[i].device() &&
                                   g[i].sizes() == p[i].sizes(), "AdamW: a gradient needs its parameter's type, device and shape, and no sparse layout");
-            TORCH_CHECK(p[i].is_cuda(), "AdamW: parameters must be on a GPU; there is no CPU fallback");
+            const uintptr_t at = (uintptr_t)p[i].data_ptr();
+            if (p[i].numel()) spans.push_back({at, at + p[i].nbytes()});
             const int64_t n = p[i].numel(), blocks = (n + VSV_ADAMW_BLOCK - 1) / VSV_ADAMW_BLOCK;
             state_fits(p[i], m[i], bits == 8 ? at::kChar : at::kFloat, n);
             state_fits(p[i], v[i], bits == 8 ? at::kByte : at::kFloat, n);
             if (bits == 8) { state_fits(p[i], ms[i], at::kFloat, blocks); state_fits(p[i], vs[i], at::kFloat, blocks); }
-            g[i] = g[i].contiguous();
+        }
+    }
+    apart(spans);
+    for (auto& call : calls) {
+        auto& [p, g, m, v, ms, vs, lr, b1, b2, eps, wd, step] = call;
+        for (size_t i = 0; i < p.size(); ++i) {
+            TORCH_CHECK(p[i].is_cuda(), "AdamW: parameters must be on a GPU; there is no CPU fallback");
+            for (const Tensor& t : {p[i], m[i], v[i]}) t.unsafeGetTensorImpl()->bump_version();
+            g[i] = g[i].resolve_neg().contiguous();
         }
     }
     for (auto& [p, g, m, v, ms, vs, lr, b1, b2, eps, wd, step] : calls) {
@@ -403,7 +425,6 @@ void adamw_step(int bits, std::vector<AdamwCall> calls) {
                 done[i] = 1;
                 table.push_back({p[i].data_ptr(), g[i].data_ptr(), m[i].data_ptr(), v[i].data_ptr(), bits == 8 ? ptr<float>(ms[i]) : nullptr,
                                  bits == 8 ? ptr<float>(vs[i]) : nullptr, (long)p[i].numel()});
-                for (const Tensor& t : {p[i], m[i], v[i]}) t.unsafeGetTensorImpl()->bump_version();
             }
             c10::DeviceGuard guard(p[first].device());
             check(api.adamw_multi(table.data(), (int)table.size(), type_code(p[first]), bits, lr, b1, b2, eps, wd, step, stream_of(p[first])),

@@ -41,6 +41,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: bad hyper-parameters lr={lr} betas={g['betas']} eps={eps} weight_decay={wd}")
             if g["state_bits"] != self.state_bits:
                 raise ValueError("AdamW: all groups hold their moments in the same number of bits")
+            if len(set(map(id, g["params"]))) < len(g["params"]):
+                raise ValueError("AdamW: a parameter is in its group twice")
             for p in g["params"]:
                 _check_param(p)
         except Exception:
