@@ -263,13 +263,15 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
 // taken for a tile at a time.
 //   A wave runs along time alone, so where sequences and channels make fewer waves than the chip has SIMDs the time axis is
 // split (scan_plan).  A first pass gives every segment's state from zero and its sum of delta; the state in front of a
-// segment then follows from exp(a sum delta), one step per earlier segment, at the start of the second pass.
+// segment then follows from exp(a sum delta), one step per earlier segment: at the start of the second pass or, of many
+// segments, between the two.
 constexpr int kTile = 8;             // steps per tile; training keeps the state before every tile
 
 struct ScanPlan {
     long seg;                        // steps per segment, a multiple of kTile
     int S;                           // segments
     int P;                           // lanes that share a channel's states (forward; then S = 1)
+    bool joined;                     // the states in front of the segments come from ssm_join_kernel
 };
 
 struct ScanPos {
@@ -277,7 +279,7 @@ struct ScanPos {
     int s;
     unsigned lane;                   // channel base + lane
     int part;                        // which R / P of its states this lane owns
-    bool live, writes;               // a channel of its own; and the one of its lanes that stores the channel's outputs
+    bool live;                       // a channel of its own
 };
 
 __device__ inline long seq_len_s(const int* lengths, long b, long T) {
@@ -300,7 +302,6 @@ template <int P = 1> __device__ inline ScanPos scan_pos(const vsv_ssm_desc& a, c
     const unsigned left = Dg - c * kCh;
     p.part = threadIdx.x / kCh;
     p.live = ch < left;
-    p.writes = p.live && p.part == 0;
     p.lane = p.live ? ch : left - 1;
     const long len = seq_len_s(a.lengths, p.b, a.T);
     p.t0 = p.s * pl.seg;
@@ -408,7 +409,7 @@ template <typename T> __device__ inline void tile_values(const T (&r)[kTile], in
 // (a dead lane's offset lies behind the buffer's end, where stores are dropped)
 template <typename T> __device__ inline void tile_store(T* row, long D, const ScanPos& p, int left, const float (&v)[kTile]) {
     const auto r = __builtin_amdgcn_make_buffer_rsrc(row, 0, 0x7fffffff, 0x00020000);
-    const int voff = p.writes ? (int)(p.lane * (unsigned)sizeof(T)) : (int)0xfffffff0;
+    const int voff = p.live ? (int)(p.lane * (unsigned)sizeof(T)) : (int)0xfffffff0;
     const int step = (int)(D * (long)sizeof(T));
 #pragma unroll
     for (int i = 0; i < kTile; ++i) {
@@ -452,32 +453,107 @@ template <int R> __device__ inline void load_decay(const vsv_ssm_desc& a, long d
     for (int n = 0; n < R; ++n) A2[n] = n0 + n < a.N ? a.a[d * a.N + n0 + n] * kLog2e : 0.0f;
 }
 
-// The sum over a channel's P lanes, which are 64 / P apart.
-template <int P> __device__ inline float part_sum(float v) {
-    static_assert(P == 1 || P == 2 || P == 4, "");
-    if constexpr (P >= 2) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-        const unsigned r0 = r[0], r1 = r[1];
-        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
-    }
+// Between the P lanes of a channel, 64 / P apart, of which lane `part` owns steps part kTile / P + j of a tile: values of the
+// own steps to all steps' in every lane, and every lane's shares of all steps to the own steps' sums.
+__device__ inline void swap32(float a, float b, float& r0, float& r1) {   // (a.lo, b.lo), (a.hi, b.hi) of the wave's halves
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned x = r[0], y = r[1];
+    r0 = __builtin_bit_cast(float, x);
+    r1 = __builtin_bit_cast(float, y);
+}
+__device__ inline void swap16(float a, float b, float& r0, float& r1) {   // the same within each half
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned x = r[0], y = r[1];
+    r0 = __builtin_bit_cast(float, x);
+    r1 = __builtin_bit_cast(float, y);
+}
+template <int P> __device__ inline void to_all(const float (&own)[kTile / P], float (&all)[kTile]) {
+    static_assert(P == 2 || P == 4, "");
+    float h[kTile / 2];
     if constexpr (P == 4) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-        const unsigned r0 = r[0], r1 = r[1];
-        v = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+#pragma unroll
+        for (int j = 0; j < kTile / 4; ++j) swap16(own[j], own[j], h[j], h[j + kTile / 4]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kTile / 2; ++j) h[j] = own[j];
     }
-    return v;
+#pragma unroll
+    for (int j = 0; j < kTile / 2; ++j) swap32(h[j], h[j], all[j], all[j + kTile / 2]);
+}
+template <int P> __device__ inline void sums_to_own(const float (&all)[kTile], float (&own)[kTile / P]) {
+    float h[kTile / 2], u, v;
+#pragma unroll
+    for (int j = 0; j < kTile / 2; ++j) { swap32(all[j], all[j + kTile / 2], u, v); h[j] = u + v; }
+    if constexpr (P == 4) {
+#pragma unroll
+        for (int j = 0; j < kTile / 4; ++j) { swap16(h[j], h[j + kTile / 4], u, v); own[j] = u + v; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kTile / 2; ++j) own[j] = h[j];
+    }
 }
 
-// v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to
+// v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to; the loads of kAhead of them are
+// under way at a time.
 template <int R>
 __device__ inline void fold_segments(const float* E, const float* sd, long D, long d, long row0, int from, int to, int step,
                                      const float (&A2)[R], float (&v)[R]) {
-    for (int k = from; k != to; k += step) {
-        float e[R];
-        load_states<R>(E + (row0 + k) * R * D, D, d, e);
-        const float s = sd[(row0 + k) * D + d];
+    constexpr int kAhead = 4;
+    const int n = (to - from) * step;
+    for (int i = 0; i < n; i += kAhead) {
+        float e[kAhead][R], s[kAhead];
 #pragma unroll
-        for (int n = 0; n < R; ++n) v[n] = __builtin_fmaf(exp2_fast(s * A2[n]), v[n], e[n]);
+        for (int u = 0; u < kAhead; ++u) {
+            const long k = row0 + from + (i + u < n ? i + u : n - 1) * step;
+            load_states<R>(E + k * R * D, D, d, e[u]);
+            s[u] = sd[k * D + d];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            pin(s[u]);
+#pragma unroll
+            for (int m = 0; m < R; ++m) pin(e[u][m]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (i + u >= n) break;
+            float w[R];
+            decays<R>(s[u], A2, w);
+#pragma unroll
+            for (int m = 0; m < R; ++m) v[m] = __builtin_fmaf(w[m], v[m], e[u][m]);
+        }
+    }
+}
+
+// The same for many segments, in a launch between the passes: E becomes the state in front of every segment (behind it,
+// backwards), so that a segment does not walk over all the others'.  A lane has one state of a channel.
+template <int R>
+__global__ void __launch_bounds__(64) ssm_join_kernel(const float* __restrict__ a, const float* __restrict__ init, int N, long D, long rows,
+                                                      int S, bool back, float* __restrict__ E, const float* __restrict__ sd) {
+    constexpr int kAhead = 16;
+    const long id = (long)blockIdx.x * 64 + threadIdx.x;
+    if (id >= rows * R * D) return;
+    const long b = id / (R * D), at = id - b * R * D, k = at / (4 * D), d = (at - k * 4 * D) >> 2;
+    const int n = (int)(k * 4 + (at & 3));
+    const float A2 = n < N ? a[d * N + n] * kLog2e : 0.0f;
+    float v = n < N && init ? init[(b * D + d) * N + n] : 0.0f;
+    for (int i = 0; i < S; i += kAhead) {
+        float e[kAhead], s[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int j = i + u < S - 1 ? i + u : S - 2;
+            const long row = b * S + (back ? S - 1 - j : j);
+            e[u] = E[row * R * D + at];
+            s[u] = sd[row * D + d];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) { pin(e[u]); pin(s[u]); }         // (all of them under way, none loaded behind the break)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (i + u >= S) break;
+            E[(b * S + (back ? S - 1 - i - u : i + u)) * R * D + at] = v;
+            v = __builtin_fmaf(exp2_fast(s[u] * A2), v, e[u]);
+        }
     }
 }
 
@@ -529,15 +605,14 @@ __global__ void __launch_bounds__(64) ssm_ends_kernel(const vsv_ssm_desc a, cons
     sd[(p.b * pl.S + p.s) * D + d] = sum;
 }
 
-// P > 1: a channel's states are shared by P lanes, R / P each, and one pass runs over all of time.
-template <typename T, int R, int P>
+// The outputs, from the state in front of the segment on.
+template <typename T, int R>
 __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, const ScanPlan pl, const float* __restrict__ E,
                                                       const float* __restrict__ sd) {
     __shared__ alignas(16) float lds[2][kTile * 2 * R];
-    constexpr int L = R / P;
-    const ScanPos p = scan_pos<P>(a, pl, blockIdx.x, 0);
+    const ScanPos p = scan_pos(a, pl, blockIdx.x, 0);
     const long D = a.D, d = p.base + p.lane;
-    const int N = a.N, n0 = p.part * L;
+    const int N = a.N;
     T* y = (T*)a.y + p.b * a.T * D + p.base;
     const T *x = (const T*)a.x + p.b * a.x_bs + p.base + p.t0 * a.x_ts, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + p.t0 * a.dt_ts;
     const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base + p.t0 * a.gate_ts : nullptr;
@@ -550,12 +625,13 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
         if (gate) load_tile(gate, (int)(a.gate_ts * (long)sizeof(T)), p.lane, left, gr);
     };
     if (p.t0 < p.t1) fetch(tile_left(p, p.t0));
-    float A2[L], h[L];
-    load_decay<L>(a, d, A2, n0);
+    float A2[R], h[R];
+    load_decay<R>(a, d, A2);
 #pragma unroll
-    for (int n = 0; n < L; ++n) h[n] = n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
-    if constexpr (P == 1) fold_segments<R>(E, sd, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
-    const float skip = a.skip && p.part == 0 ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
+    for (int n = 0; n < R; ++n) h[n] = n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n] : 0.0f;
+    if (pl.joined) load_states<R>(E + (p.b * pl.S + p.s) * R * D, D, d, h);
+    else fold_segments<R>(E, sd, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
+    const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     float* saved = a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D : nullptr;
     int buf = 0;
     for (long t = p.t0; t < p.t1; t += kTile, buf ^= 1) {
@@ -574,25 +650,25 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
             fetch(tile_left(p, t + kTile));
         }
         if (saved) {
-            if (p.live) store_states<L>(saved + n0 * D, D, d, h);
+            if (p.live) store_states<R>(saved, D, d, h);
             saved += R * D;
         }
         order();
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            float b[L], c[L], e[L], acc[2] = {skip * xv[i], 0.0f};
-            bc_row<L>(lds[buf] + i * 2 * R + n0, b);
-            bc_row<L>(lds[buf] + i * 2 * R + R + n0, c);
+            float b[R], c[R], e[R], acc[2] = {skip * xv[i], 0.0f};
+            bc_row<R>(lds[buf] + i * 2 * R, b);
+            bc_row<R>(lds[buf] + i * 2 * R + R, c);
             const float dx = de[i] * xv[i];
-            decays<L>(de[i], A2, e);
-            if constexpr (P == 1) order();
+            decays<R>(de[i], A2, e);
+            order();
 #pragma unroll
-            for (int n = 0; n < L; ++n) {
+            for (int n = 0; n < R; ++n) {
                 h[n] = __builtin_fmaf(e[n], h[n], dx * b[n]);
                 acc[n & 1] = __builtin_fmaf(c[n], h[n], acc[n & 1]);
             }
-            yv[i] = part_sum<P>(acc[0] + acc[1]);
-            if constexpr (P == 1) order();                               // (few states: steps side by side fit the registers)
+            yv[i] = acc[0] + acc[1];
+            order();
         }
         if (gate) {
 #pragma unroll
@@ -600,9 +676,102 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
         }
         tile_store(y + t * D, D, p, left, yv);
     }
-    if (p.writes)
+    if (p.live)
         for (long t = p.t0 > p.t1 ? p.t0 : p.t1; t < p.tz; ++t) (y + t * D)[p.lane] = from_f<T>(0.0f);
     if (a.state_out && p.live && p.s == pl.S - 1)
+#pragma unroll
+        for (int n = 0; n < R; ++n)
+            if (n < N) a.state_out[(p.b * D + d) * N + n] = h[n];
+}
+
+// Short sequences of few waves: P = R / 4 lanes share a channel, four states each, and one pass runs over all of time.  A wave
+// is alone on its SIMD and every instruction counts, so a tile's steps are shared too: a lane loads, activates, gates and stores
+// kTile / P of them.
+template <typename T, int R, int P>
+__global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, const ScanPlan pl) {
+    __shared__ alignas(16) float lds[2][kTile * 2 * R];
+    constexpr int L = R / P, O = kTile / P;
+    constexpr unsigned kSize = sizeof(T);
+    const ScanPos p = scan_pos<P>(a, pl, blockIdx.x, 0);
+    const long D = a.D, d = p.base + p.lane;
+    const int N = a.N, n0 = p.part * L, own = p.part * O;                 // the first of this lane's states and steps
+    const T *x = (const T*)a.x + p.b * a.x_bs + p.base, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base;
+    const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base : nullptr;
+    T* y = (T*)a.y + p.b * a.T * D + p.base;
+    const unsigned x_step = (unsigned)a.x_ts * kSize, dt_step = (unsigned)a.dt_ts * kSize, gate_step = (unsigned)a.gate_ts * kSize;
+    BcTile<T, R> bc(a, p, 0, true, true);
+    T xr[O], dr[O], gr[O];
+    auto fetch = [&](int left) {                                          // rows behind the first `left` repeat the last
+        bc.fetch(N, left);
+        const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(x), 0, -1, 0x00020000);
+        const auto rd = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(dt), 0, -1, 0x00020000);
+        const auto rg = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(gate), 0, -1, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < O; ++j) {
+            const unsigned row = own + j < left ? own + j : left - 1, at = p.lane * kSize;
+            xr[j] = buffer_get<T>(rx, row * x_step + at, 0);
+            dr[j] = buffer_get<T>(rd, row * dt_step + at, 0);
+            if (gate) gr[j] = buffer_get<T>(rg, row * gate_step + at, 0);
+        }
+    };
+    if (p.t1 > 0) fetch(tile_left(p, 0));
+    float A2[L], h[L];
+    load_decay<L>(a, d, A2, n0);
+#pragma unroll
+    for (int n = 0; n < L; ++n) h[n] = n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
+    const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
+    float* saved = a.saved ? a.saved + p.b * ((a.T + kTile - 1) / kTile) * R * D + n0 * D : nullptr;
+    int buf = 0;
+    for (long t = 0; t < p.t1; t += kTile, buf ^= 1) {
+        const int left = tile_left(p, t);
+        float xv[O], gv[O], de_own[O], dx_own[O], de[kTile], dx[kTile], yv[kTile], out[O];
+        bc.lay(lds[buf]);
+#pragma unroll
+        for (int j = 0; j < O; ++j) {
+            const float raw = to_f(dr[j]) + dtb, s = a.softplus ? softplus_f(raw) : raw;
+            xv[j] = to_f(xr[j]);
+            gv[j] = gate ? to_f(gr[j]) : 1.0f;
+            if (gate) gv[j] *= sigmoid_f(gv[j]);
+            de_own[j] = own + j < left ? s : 0.0f;                        // (delta = 0 leaves every state as it is)
+            dx_own[j] = own + j < left ? s * xv[j] : 0.0f;
+        }
+        if (t + kTile < p.t1) {
+            x += kTile * a.x_ts; dt += kTile * a.dt_ts; gate += gate ? kTile * a.gate_ts : 0; bc.move(1);
+            fetch(tile_left(p, t + kTile));
+        }
+        if (saved) {
+            if (p.live) store_states<L>(saved, D, d, h);
+            saved += R * D;
+        }
+        to_all<P>(de_own, de);
+        to_all<P>(dx_own, dx);
+        order();
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+            float b[L], c[L], e[L], acc[2] = {};
+            bc_row<L>(lds[buf] + i * 2 * R + n0, b);
+            bc_row<L>(lds[buf] + i * 2 * R + R + n0, c);
+            decays<L>(de[i], A2, e);
+#pragma unroll
+            for (int n = 0; n < L; ++n) {
+                h[n] = __builtin_fmaf(e[n], h[n], dx[i] * b[n]);
+                acc[n & 1] = __builtin_fmaf(c[n], h[n], acc[n & 1]);
+            }
+            yv[i] = acc[0] + acc[1];
+        }
+        sums_to_own<P>(yv, out);
+        const auto ry = __builtin_amdgcn_make_buffer_rsrc(y + t * D, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < O; ++j) {
+            const T o = from_f<T>(__builtin_fmaf(skip, xv[j], out[j]) * gv[j]);
+            const unsigned at = p.live && own + j < left ? (unsigned)(own + j) * (unsigned)D * kSize + p.lane * kSize : 0xfffffff0u;
+            if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, o), ry, (int)at, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, o), ry, (int)at, 0, 0);
+        }
+    }
+    if (p.live)
+        for (long t = p.t1 + p.part; t < a.T; t += P) (y + t * D)[p.lane] = from_f<T>(0.0f);
+    if (a.state_out && p.live)
 #pragma unroll
         for (int n = 0; n < L; ++n)
             if (n0 + n < N) a.state_out[(p.b * D + d) * N + n0 + n] = h[n];
@@ -684,15 +853,15 @@ template <int NV> __device__ inline float wave_sums(float (&v)[NV]) {
     static_assert(NV == 8 || NV == 16 || NV == 32, "");
 #pragma unroll
     for (int j = 0; j < NV / 2; ++j) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[j]), __builtin_bit_cast(unsigned, v[j + NV / 2]), false, false);
-        const unsigned r0 = r[0], r1 = r[1];
-        v[j] = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+        float r0, r1;
+        swap32(v[j], v[j + NV / 2], r0, r1);
+        v[j] = r0 + r1;
     }
 #pragma unroll
     for (int j = 0; j < NV / 4; ++j) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v[j]), __builtin_bit_cast(unsigned, v[j + NV / 4]), false, false);
-        const unsigned r0 = r[0], r1 = r[1];
-        v[j] = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+        float r0, r1;
+        swap16(v[j], v[j + NV / 4], r0, r1);
+        v[j] = r0 + r1;
     }
     const int l = threadIdx.x;
     if constexpr (NV >= 8) halve<kRor8, NV / 8>(v, l & 8);
@@ -727,7 +896,8 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
     load_decay<R>(a, d, A2);
 #pragma unroll
     for (int n = 0; n < R; ++n) q[n] = n < N && gr.d_state_out ? gr.d_state_out[(p.b * D + d) * N + n] : 0.0f;
-    fold_segments<R>(E, sd, D, d, p.b * pl.S, pl.S - 1, p.s, -1, A2, q);
+    if (pl.joined) load_states<R>(E + (p.b * pl.S + p.s) * R * D, D, d, q);
+    else fold_segments<R>(E, sd, D, d, p.b * pl.S, pl.S - 1, p.s, -1, A2, q);
     if (!p.live) {
 #pragma unroll
         for (int n = 0; n < R; ++n) q[n] = 0.0f;
@@ -1024,10 +1194,12 @@ template <typename F> int by_states(int N, F&& f) {
 long ssm_blocks(const vsv_ssm_desc* a) { return (a->D / a->G + 63) / 64; }
 
 // How the work is divided.  A split of time costs a second pass (1.8 times the work) and a launch, so it pays below about half
-// a wave per SIMD (1024 of them): then as many segments as make two waves per SIMD, none shorter than two tiles, at most
-// kMaxSegments (the start of a segment walks over those in front of it).  Short sequences of so few waves are read forward in
-// one pass instead, with a channel's states shared by R / 4 lanes (64x60x100 float32: 26 us with one lane a channel).
-constexpr long kMaxSegments = 64, kSplitFrom = 64, kShareBelow = 192, kSplitWaves = 2048;
+// a wave per SIMD (1024 of them): then as many segments as make two waves per SIMD, none shorter than two tiles (three were
+// slower at 64x128x100 to 5x777x198), at most kMaxSegments (1x4096x256 forward and backward: 64 segments 173 us, 256 124).  A
+// few segments are folded by those behind them, many in a launch of their own (5x777x198, 48 segments, forward: 34 and 31 us;
+// 4x2048x2048, 16 segments, backward: 329 and 340).  Short sequences of so few waves are read forward in one pass instead, with
+// a channel's states shared by R / 4 lanes (64x60x100: 25 us with one lane a channel, 14 us; 64x128x100: 22 us, split 22).
+constexpr long kMaxSegments = 256, kSplitFrom = 40, kJoinFrom = 24, kShareBelow = 128, kSplitWaves = 2048;
 
 ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
     ScanPlan pl = {};
@@ -1035,7 +1207,7 @@ ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
     long S = 1;
     pl.P = 1;
     if (waves > 0 && waves < 512) {
-        if (forward && a->T < kShareBelow) pl.P = padded_states(a->N) / 4;
+        if (forward && a->T < kShareBelow && a->N > 4) pl.P = padded_states(a->N) / 4;
         else if (a->T >= kSplitFrom) {
             S = (kSplitWaves + waves - 1) / waves;
             if (S > tiles / 2) S = tiles / 2;
@@ -1045,11 +1217,18 @@ ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
     const long per = tiles > 0 ? (tiles + S - 1) / S : 1;
     pl.seg = per * kTile;
     pl.S = tiles > 0 ? (int)((tiles + per - 1) / per) : 1;
+    pl.joined = pl.S >= kJoinFrom;
     return pl;
 }
 
 size_t ends_floats(const vsv_ssm_desc* a, const ScanPlan& pl) {
     return pl.S > 1 ? (size_t)a->B * pl.S * (padded_states(a->N) + 1) * a->D : 0;
+}
+template <int R> int join_segments(const vsv_ssm_desc* a, const ScanPlan& pl, const float* init, bool back, float* E, const float* sd, hipStream_t stream) {
+    if (!pl.joined) return 0;
+    const long blocks = (a->B * R * a->D + 63) / 64;                      // (split scans have fewer than 512 waves of channels)
+    hipLaunchKernelGGL(ssm_join_kernel<R>, dim3((unsigned)blocks), dim3(64), 0, stream, a->a, init, a->N, a->D, a->B, pl.S, back, E, sd);
+    return op_launch_check("ssm_join_kernel");
 }
 size_t round4(size_t n) { return (n + 3) & ~(size_t)3; }
 
@@ -1149,12 +1328,17 @@ extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, vo
         if (pl.S > 1) {
             hipLaunchKernelGGL((ssm_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
             if (int rc = op_launch_check("ssm_ends_kernel")) return rc;
+            if (int rc = join_segments<R>(a, pl, a->state_in, false, E, sd, (hipStream_t)stream)) return rc;
         }
-        if (R > 4 && pl.P > 1) {
-            constexpr int P = R / 4, kCh = 64 / P;
-            const long groups = a->B * a->G * ((a->D / a->G + kCh - 1) / kCh);
-            hipLaunchKernelGGL((ssm_scan_kernel<T, R, P>), dim3((unsigned)groups), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
-        } else hipLaunchKernelGGL((ssm_scan_kernel<T, R, 1>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+        if constexpr (R > 4) {
+            if (pl.P > 1) {
+                constexpr int P = R / 4, kCh = 64 / P;
+                const long groups = a->B * a->G * ((a->D / a->G + kCh - 1) / kCh);
+                hipLaunchKernelGGL((ssm_shared_kernel<T, R, P>), dim3((unsigned)groups), dim3(64), 0, (hipStream_t)stream, *a, pl);
+                return op_launch_check("ssm_shared_kernel");
+            }
+        }
+        hipLaunchKernelGGL((ssm_scan_kernel<T, R>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
         return op_launch_check("ssm_scan_kernel");
     }); });
 }
@@ -1193,6 +1377,7 @@ extern "C" int vsv_ssm_scan_backward(const vsv_ssm_desc* a, const vsv_ssm_grads*
             if (pl.S > 1) {
                 hipLaunchKernelGGL((ssm_bwd_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd);
                 if (int rc = op_launch_check("ssm_bwd_ends_kernel")) return rc;
+                if (int rc = join_segments<R>(a, pl, g->d_state_out, true, E, sd, (hipStream_t)stream)) return rc;
             }
             hipLaunchKernelGGL((ssm_bwd_kernel<T, R>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, *g, pl, E, sd, pbc, pp);
             return op_launch_check("ssm_bwd_kernel");
