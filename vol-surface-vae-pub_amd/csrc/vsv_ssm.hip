@@ -15,8 +15,8 @@ __device__ inline long seq_len(const int* lengths, long b, long T) {
 // ---- short causal convolution ------------------------------------------------------------------------------------
 // One output from the window, tap by tap and each operation rounded by itself: a prompt and the tokens behind it come out
 // bit for bit the same, whichever kernel computes them, and so does any evaluation that takes the formula at its word -- what
-// is rounded to 16 bits here feeds a recurrent state.  The exponential is the accurate one; the quotient 1 / (1 + e) is the
-// reciprocal with one Newton step (a full division costs ten operations more).
+// is rounded to 16 bits here feeds a recurrent state.  exp(-s) is 2^t with what t = -s log2 e is rounded by put behind it; the
+// quotient 1 / (1 + e) is the reciprocal with one Newton step (a full division costs ten operations more).
 template <int K>
 __device__ inline float conv_pre(const float (&w)[K], const float (&x)[K], float bias) {
 #pragma clang fp contract(off)
@@ -26,7 +26,10 @@ __device__ inline float conv_pre(const float (&w)[K], const float (&x)[K], float
     return s + bias;
 }
 __device__ inline float conv_silu(float s) {
-    const float y = __builtin_fminf(1.0f + expf(-s), 3e38f), r = __builtin_amdgcn_rcpf(y);
+    constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f, kLn2 = 0.693147182f;       // log2 e, what it is rounded by, 1 / log2 e
+    const float x = __builtin_amdgcn_fmed3f(-s, -100.0f, 100.0f), t = x * kHi;
+    const float e = exp2_fast(t) * __builtin_fmaf(__builtin_fmaf(x, kLo, __builtin_fmaf(x, kHi, -t)), kLn2, 1.0f);
+    const float y = __builtin_fminf(1.0f + e, 3e38f), r = __builtin_amdgcn_rcpf(y);
     return s * __builtin_fmaf(__builtin_fmaf(-y, r, 1.0f), r, r);
 }
 
