@@ -498,3 +498,32 @@ def test_states_made_in_inference_mode():
         mem.step(x[:, 8], state)
     torch.cuda.synchronize()
     assert all(torch.equal(t, k) for t, k in zip(state, kept))
+
+
+@pytest.mark.parametrize("T, N, lengths", [(600, 16, [600, 17, 0]), (600, 8, [8, 591, 592]), (47, 16, [47, 40, 3]), (100, 4, [100, 41, 0]),
+                                           (2100, 3, [2100, 2097, 1000]), (127, 5, [127, 120, 9])])
+def test_scan_padded_in_many_segments(T, N, lengths):
+    """Lengths that end in the first, a middle, the last or in front of every segment."""
+    s = _scan_case(44, 3, T, 70, N, 1, "fp32")
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    s["x"][torch.arange(T).cuda()[None, :] >= n[:, None]] = float("nan")
+    _scan_check(s, _scan_run(s, n), n)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("N", [4, 8, 16])
+def test_step_with_b_and_c_anywhere(N, dtype):
+    """b and c as pieces of a projection whose rows start on any element."""
+    from vsv.ssm import ssm_step
+    s = _scan_case(45, 5, 1, 70, N, 2, dtype)
+    x, dt, gate, b, c = (s[k][:, 0] for k in ("x", "dt", "gate", "b", "c"))
+    states, ys = [], []
+    for at, end in ((0, 0), (1, 0), (3, 2), (4, 4)):
+        row = torch.cat([torch.full((5, at), 7.0, device="cuda", dtype=b.dtype), b.flatten(1), c.flatten(1),
+                         torch.full((5, end), 7.0, device="cuda", dtype=b.dtype)], 1)
+        _, vb, vc, _ = row.split([at, 2 * N, 2 * N, end], 1)
+        states.append(s["h0"].clone())
+        ys.append(ssm_step(x, dt, s["a"], vb.unflatten(1, (2, N)), vc.unflatten(1, (2, N)), s["skip"], gate, state=states[-1], dt_bias=s["dt_bias"]))
+    for y, st in zip(ys, states):
+        _scan_check(s, {"y": y[:, None], "state": st})
+        assert torch.equal(y, ys[0]) and torch.equal(st, states[0])
