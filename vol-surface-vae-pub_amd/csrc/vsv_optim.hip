@@ -35,6 +35,7 @@ __device__ inline int tensor_of(const Table& tab, unsigned blk) {
 }
 
 // ---- 32 bits -----------------------------------------------------------------------------------------------------
+// 168 M float32 parameters: 883 us, 5.3 TB/s.  Eight elements a thread, all loads ahead.
 constexpr int kPer32 = 4, kIter32 = 2, kChunk32 = 256 * kPer32 * kIter32;
 
 __device__ inline void update32(float& p, float g, float& m, float& v, const Hyper& h) {
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__(256) adamw32_kernel(const Table tab, const Hyp
 // additive (Weyl) sequence over steps and elements (for v, 1 - u).  Over steps u is spread evenly, so the rounding is
 // unbiased in time; to the nearest code, v would never move: beta2 = 0.999 changes it by 0.1 % a step, codes are at least
 // 1.6 % apart.  v > 0 never becomes 0, which would leave m without its divisor.
+//   168 M bf16 parameters: 441 to 461 us, the issue of 90 vector operations an element (2.4 GB at the copy rate: 350 us).
 //   The moments are computed in 64 bits (full rate on this chip), and so is the choice of a code wherever float32 could
 // choose another: the codes are the definition's, not a rounding away from it.
 //   A gradient that is not finite leaves its element's moments alone and makes the parameter NaN: a NaN scale would take
@@ -253,7 +255,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const Table tab, const Hype
     if (threadIdx.x % kLanes8 == 0) { e.m_scale[blk] = sm; e.v_scale[blk] = sv; }
 }
 
-// The values that the codes stand for, in float32: t.p and t.g are the two outputs here.
+// The values that the codes stand for, in float32: t.p and t.g are the two outputs here (four fifths of its bytes are writes:
+// 168 M elements 240 to 340 us).
 __global__ void __launch_bounds__(256) adamw8_read_kernel(const Table tab) {
     const int ti = tensor_of(tab, blockIdx.x);
     const vsv_adamw_tensor& e = tab.t[ti];

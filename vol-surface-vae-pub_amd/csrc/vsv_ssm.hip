@@ -34,9 +34,9 @@ __device__ inline float conv_silu(float s) {
 }
 
 // pre[t,d] = bias[d] + sum_k w[d,k] xs[t-K+1+k, d],  y = silu(pre) or pre; xs is x, continued into state_in before t = 0.
-// One read of x and one write of y (2K flops an element): bound by memory.  A thread owns VEC neighbouring channels and a
-// chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it works on kRows rows at a
-// time, with the next ones under way.
+// One read of x and one write of y (2K flops an element): bound by memory (8x2048x4096 bf16: 66 us, 4.0 TB/s).  A thread owns VEC
+// neighbouring channels and a chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it
+// works on kRows rows at a time, with the next ones under way.
 template <typename T, int K, int VEC, int kRows> struct ConvRows {
     const T* x;                      // the sequence's row 0, at this thread's channels
     const float* st;                 // state_in's, or null
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
 
 // ds = dy act'(pre) (pre computed again from x), dx[t] = sum_k w[k] ds[t+K-1-k], dw[k] = sum_t ds[t] xs[t-K+1+k],
 // dbias = sum_t ds.  The same chunks; a chunk reads K-1 rows beyond each end, its sums over time go to `part`
-// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.
+// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.  8x2048x4096 bf16: 105 us, 3.8 TB/s.
 template <typename T, int K, int VEC, int kRows>
 __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_conv_desc a, const vsv_short_conv_grads g, long chunk, long n_chunk,
                                                              long n_vec, float* __restrict__ part) {
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
 // delta = softplus(dt + dt_bias),  h_t = exp(delta a) h_{t-1} + delta x b_t,  y = (c_t . h_t + skip x) silu(gate).
 // The decay belongs to (channel, state), so there is no matrix form: per state and step one exponential and four float32
 // operations, 24 cycles of a SIMD per 64 channels, against 8 bytes of traffic per channel and step in 16 bits.  Bound by
-// the vector units.
+// the vector units: 1x16384x2048 bf16 takes 261 us in all, of which the issue of its vector instructions is 227.
 //   A lane owns a channel and its N states (padded to R) in registers, a wave 64 channels of one group, which share b_t and
 // c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are computed; the activations are
 // taken for a tile at a time.
@@ -876,7 +876,7 @@ template <int NV> __device__ inline float wave_sums(float (&v)[NV]) {
 // A tile at a time from the state saved in front of it: its states are computed again into registers, then q runs through
 // them in reverse, four states at a time so that they fit.  The gradients of b and c are sums over channels: over the
 // wave's 64 here, over the channel blocks in ssm_sums_kernel; those of a, skip and dt_bias sums over time: here, and over
-// sequences and segments there too.  All in a fixed order.
+// sequences and segments there too.  All in a fixed order.  4x2048x2048 bf16: 273 us, vector units at two waves a SIMD.
 template <typename T, int R>
 __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, const vsv_ssm_grads gr, const ScanPlan pl, const float* __restrict__ E,
                                                         const float* __restrict__ sd, float* __restrict__ part_bc, float* __restrict__ part_p) {
@@ -1141,7 +1141,7 @@ bool conv_words(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, siz
     return ok;
 }
 // Channels per thread: four where the rows allow it; backward eight in 16 bits (two rows under way instead of four fit the
-// registers: 8x2048x4096 bf16 108 us for 131; forward they are slower, 85 for 74).
+// registers: 8x2048x4096 bf16 108 us for 131; forward they are slower, 80 for 67).
 int conv_vec(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g) {
     const size_t size = a->dtype == VSV_F32 ? 4 : 2;
     if (g && size == 2 && conv_words(a, g, size, 8)) return 8;
@@ -1149,8 +1149,8 @@ int conv_vec(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g) {
 }
 
 // Time steps per thread: the longer, the less is read twice and the fewer sums are left over, as long as the threads fill the
-// chip.  Forward eight waves for every SIMD (8x2048x4096 bf16: two 87, four 77, eight 74 us); backward, where a chunk leaves K + 1
-// sums per channel, two (131 us, four 138).
+// chip.  Forward eight waves for every SIMD (8x2048x4096 bf16: two 69 us, eight 66, sixteen 68); backward, where a chunk leaves
+// K + 1 sums per channel, two (108 us and 5 for the sums; one 157, four 120 and 11).
 constexpr long kConvFill = 524288, kConvBwdFill = 131072;
 long conv_chunk(const vsv_short_conv_desc* a, long fill, long vec) {
     const long rows = a->B * (a->D / vec);

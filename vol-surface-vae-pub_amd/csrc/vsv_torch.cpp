@@ -2,6 +2,7 @@
 // functions over the C entries (include/vsv_hip.h).  Native because a call of theirs takes the GPU a few microseconds: the
 // same code in Python took the host 45 us forward and 60 us backward (on top of what autograd itself takes).
 // The C entries' addresses come from the library that vsv/lib.py has loaded (bind), so there is one copy of it.
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -116,14 +117,16 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
 
 Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+// (straight from the allocator: through the dispatcher a tensor costs the host twice as much, and a backward pass makes twelve)
+Tensor fresh(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) { return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt)); }
+Tensor whole_like(const Tensor& t) { return fresh(t, t.sizes(), t.scalar_type()); }
+Tensor floats(const Tensor& like, at::IntArrayRef shape) { return fresh(like, shape, at::kFloat); }
+Tensor workspace(const Tensor& like, size_t bytes) { return fresh(like, {(int64_t)(bytes ? bytes : 16)}, at::kByte); }
 // what a backward pass returns for an input: nothing where no gradient was asked for
-Tensor grad_like(const Tensor& input) { return input.defined() && input.requires_grad() ? at::empty_like(input) : Tensor(); }
+Tensor grad_like(const Tensor& input) { return input.defined() && input.requires_grad() ? whole_like(input) : Tensor(); }
 Tensor asked(const Tensor& input, const Tensor& grad) { return input.defined() && input.requires_grad() ? grad : Tensor(); }
 
 template <typename T = void> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
-Tensor whole_like(const Tensor& t) { return at::empty_like(t, t.options(), at::MemoryFormat::Contiguous); }
-Tensor floats(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
-Tensor workspace(const Tensor& like, size_t bytes) { return at::empty({(int64_t)(bytes ? bytes : 16)}, like.options().dtype(at::kByte)); }
 
 // With create_graph the gradients carry an error for whoever differentiates them again.
 variable_list once(variable_list grads, const char* what) {
@@ -436,8 +439,8 @@ void adamw_step(int bits, std::vector<AdamwCall> calls) {
 std::pair<Tensors, Tensors> adamw_read8(const Tensors& m, const Tensors& v, const Tensors& ms, const Tensors& vs) {
     Tensors mo, vo;
     for (const Tensor& t : m) {
-        mo.push_back(at::empty(t.sizes(), t.options().dtype(at::kFloat)));
-        vo.push_back(at::empty(t.sizes(), t.options().dtype(at::kFloat)));
+        mo.push_back(floats(t, t.sizes()));
+        vo.push_back(floats(t, t.sizes()));
     }
     std::vector<char> done(m.size(), 0);
     for (size_t first = 0; first < m.size(); ++first) {
