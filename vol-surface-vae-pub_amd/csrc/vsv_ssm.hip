@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
 // The decay belongs to (channel, state), so there is no matrix form: per state and step one exponential and four float32
 // operations, 24 cycles of a SIMD per 64 channels, against 8 bytes of traffic per channel and step in 16 bits.  Bound by
 // the vector units: 1x16384x2048 bf16 takes 261 us in all, of which the issue of its vector instructions is 227.
-//   A lane owns a channel and its N states (padded to R) in registers, a wave 64 channels of one group, which share b_t and
-// c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are computed; the activations are
+//   A lane owns a channel and its N states (padded to R) in registers (or four of them), a wave 64 channels of one group (or
+// 256 / R), which share b_t and c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are computed; the activations are
 // taken for a tile at a time.
 //   A wave runs along time alone, so where sequences and channels make fewer waves than the chip has SIMDs the time axis is
 // split (scan_plan).  A first pass gives every segment's state from zero and its sum of delta; the state in front of a
@@ -273,7 +273,7 @@ constexpr int kTile = 8;             // steps per tile; training keeps the state
 struct ScanPlan {
     long seg;                        // steps per segment, a multiple of kTile
     int S;                           // segments
-    int P;                           // lanes that share a channel's states (forward; then S = 1)
+    int P;                           // lanes that share a channel's states (forward)
     bool joined;                     // the states in front of the segments come from ssm_join_kernel
 };
 
@@ -499,7 +499,7 @@ template <int P> __device__ inline void sums_to_own(const float (&all)[kTile], f
 // v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to; the loads of kAhead of them are
 // under way at a time.
 template <int R>
-__device__ inline void fold_segments(const float* E, const float* sd, long D, long d, long row0, int from, int to, int step,
+__device__ inline void fold_segments(const float* E, const float* sd, long row_floats, long D, long d, long row0, int from, int to, int step,
                                      const float (&A2)[R], float (&v)[R]) {
     constexpr int kAhead = 4;
     const int n = (to - from) * step;
@@ -508,7 +508,7 @@ __device__ inline void fold_segments(const float* E, const float* sd, long D, lo
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const long k = row0 + from + (i + u < n ? i + u : n - 1) * step;
-            load_states<R>(E + k * R * D, D, d, e[u]);
+            load_states<R>(E + k * row_floats, D, d, e[u]);
             s[u] = sd[k * D + d];
         }
 #pragma unroll
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
 #pragma unroll
     for (int n = 0; n < R; ++n) h[n] = n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n] : 0.0f;
     if (pl.joined) load_states<R>(E + (p.b * pl.S + p.s) * R * D, D, d, h);
-    else fold_segments<R>(E, sd, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
+    else fold_segments<R>(E, sd, R * D, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
     const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     float* saved = a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D : nullptr;
     int buf = 0;
@@ -687,22 +687,22 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
             if (n < N) a.state_out[(p.b * D + d) * N + n] = h[n];
 }
 
-// Short sequences of few waves: P = R / 4 lanes share a channel, four states each, and one pass runs over all of time.  A wave
-// is alone on its SIMD and every instruction counts, so a tile's steps are shared too: a lane loads, activates, gates and stores
-// kTile / P of them.
-template <typename T, int R, int P>
-__global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, const ScanPlan pl) {
+// Both passes where waves are few: P = R / 4 lanes share a channel, four states each.  A wave is alone on its SIMD and every
+// instruction counts, so a tile's steps are shared too: a lane loads, activates, gates and stores kTile / P of them.  ENDS: the
+// first pass.
+template <typename T, int R, int P, bool ENDS>
+__global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, const ScanPlan pl, float* __restrict__ E, float* __restrict__ sd) {
     __shared__ alignas(16) float lds[2][kTile * 2 * R];
     constexpr int L = R / P, O = kTile / P;
     constexpr unsigned kSize = sizeof(T);
     const ScanPos p = scan_pos<P>(a, pl, blockIdx.x, 0);
     const long D = a.D, d = p.base + p.lane;
     const int N = a.N, n0 = p.part * L, own = p.part * O;                 // the first of this lane's states and steps
-    const T *x = (const T*)a.x + p.b * a.x_bs + p.base, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base;
-    const T* gate = a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base : nullptr;
+    const T *x = (const T*)a.x + p.b * a.x_bs + p.base + p.t0 * a.x_ts, *dt = (const T*)a.dt + p.b * a.dt_bs + p.base + p.t0 * a.dt_ts;
+    const T* gate = !ENDS && a.gate ? (const T*)a.gate + p.b * a.gate_bs + p.base + p.t0 * a.gate_ts : nullptr;
     T* y = (T*)a.y + p.b * a.T * D + p.base;
     const unsigned x_step = (unsigned)a.x_ts * kSize, dt_step = (unsigned)a.dt_ts * kSize, gate_step = (unsigned)a.gate_ts * kSize;
-    BcTile<T, R> bc(a, p, 0, true, true);
+    BcTile<T, R> bc(a, p, p.t0, true, !ENDS);
     T xr[O], dr[O], gr[O];
     auto fetch = [&](int left) {                                          // rows behind the first `left` repeat the last
         bc.fetch(N, left);
@@ -717,15 +717,18 @@ __global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, co
             if (gate) gr[j] = buffer_get<T>(rg, row * gate_step + at, 0);
         }
     };
-    if (p.t1 > 0) fetch(tile_left(p, 0));
-    float A2[L], h[L];
+    if (p.t0 < p.t1) fetch(tile_left(p, p.t0));
+    float A2[L], h[L], sum = 0.0f;
+    const long segment = (p.b * pl.S + p.s) * R * D + n0 * D;
     load_decay<L>(a, d, A2, n0);
 #pragma unroll
-    for (int n = 0; n < L; ++n) h[n] = n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
+    for (int n = 0; n < L; ++n) h[n] = !ENDS && n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
+    if (!ENDS && pl.joined) load_states<L>(E + segment, D, d, h);
+    else if (!ENDS) fold_segments<L>(E + n0 * D, sd, R * D, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
     const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
-    float* saved = a.saved ? a.saved + p.b * ((a.T + kTile - 1) / kTile) * R * D + n0 * D : nullptr;
+    float* saved = !ENDS && a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D + n0 * D : nullptr;
     int buf = 0;
-    for (long t = 0; t < p.t1; t += kTile, buf ^= 1) {
+    for (long t = p.t0; t < p.t1; t += kTile, buf ^= 1) {
         const int left = tile_left(p, t);
         float xv[O], gv[O], de_own[O], dx_own[O], de[kTile], dx[kTile], yv[kTile], out[O];
         bc.lay(lds[buf]);
@@ -753,15 +756,17 @@ __global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, co
         for (int i = 0; i < kTile; ++i) {
             float b[L], c[L], e[L], acc[2] = {};
             bc_row<L>(lds[buf] + i * 2 * R + n0, b);
-            bc_row<L>(lds[buf] + i * 2 * R + R + n0, c);
+            if constexpr (!ENDS) bc_row<L>(lds[buf] + i * 2 * R + R + n0, c);
             decays<L>(de[i], A2, e);
+            if constexpr (ENDS) sum += de[i];
 #pragma unroll
             for (int n = 0; n < L; ++n) {
                 h[n] = __builtin_fmaf(e[n], h[n], dx[i] * b[n]);
-                acc[n & 1] = __builtin_fmaf(c[n], h[n], acc[n & 1]);
+                if constexpr (!ENDS) acc[n & 1] = __builtin_fmaf(c[n], h[n], acc[n & 1]);
             }
             yv[i] = acc[0] + acc[1];
         }
+        if constexpr (ENDS) continue;
         sums_to_own<P>(yv, out);
         const auto ry = __builtin_amdgcn_make_buffer_rsrc(y + t * D, 0, 0x7fffffff, 0x00020000);
 #pragma unroll
@@ -772,9 +777,14 @@ __global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, co
             else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, o), ry, (int)at, 0, 0);
         }
     }
-    if (p.live)
-        for (long t = p.t1 + p.part; t < a.T; t += P) (y + t * D)[p.lane] = from_f<T>(0.0f);
-    if (a.state_out && p.live)
+    if (!p.live) return;
+    if constexpr (ENDS) {
+        store_states<L>(E + segment, D, d, h);
+        if (p.part == 0) sd[(p.b * pl.S + p.s) * D + d] = sum;
+        return;
+    }
+    for (long t = (p.t0 > p.t1 ? p.t0 : p.t1) + p.part; t < p.tz; t += P) (y + t * D)[p.lane] = from_f<T>(0.0f);
+    if (a.state_out && p.s == pl.S - 1)
 #pragma unroll
         for (int n = 0; n < L; ++n)
             if (n0 + n < N) a.state_out[(p.b * D + d) * N + n0 + n] = h[n];
@@ -900,7 +910,7 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
 #pragma unroll
     for (int n = 0; n < R; ++n) q[n] = n < N && gr.d_state_out ? gr.d_state_out[(p.b * D + d) * N + n] : 0.0f;
     if (pl.joined) load_states<R>(E + (p.b * pl.S + p.s) * R * D, D, d, q);
-    else fold_segments<R>(E, sd, D, d, p.b * pl.S, pl.S - 1, p.s, -1, A2, q);
+    else fold_segments<R>(E, sd, R * D, D, d, p.b * pl.S, pl.S - 1, p.s, -1, A2, q);
     if (!p.live) {
 #pragma unroll
         for (int n = 0; n < R; ++n) q[n] = 0.0f;
@@ -1204,9 +1214,11 @@ long ssm_blocks(const vsv_ssm_desc* a) { return (a->D / a->G + 63) / 64; }
 // a wave per SIMD (1024 of them): then as many segments as make two waves per SIMD, none shorter than two tiles (three were
 // slower at 64x128x100 to 5x777x198), at most kMaxSegments (1x4096x256 forward and backward: 64 segments 173 us, 256 124).  A
 // few segments are folded by those behind them, many in a launch of their own (5x777x198, 48 segments, forward: 34 and 31 us;
-// 4x2048x2048, 16 segments, backward: 329 and 340).  Short sequences of so few waves are read forward in one pass instead, with
-// a channel's states shared by R / 4 lanes (64x60x100: 25 us with one lane a channel, 14 us; 64x128x100: 22 us, split 22).
-constexpr long kMaxSegments = 256, kSplitFrom = 40, kJoinFrom = 24, kShareBelow = 128, kSplitWaves = 2048;
+// 4x2048x2048, 16 segments, backward: 329 and 340).
+//   Forward, and as long as that leaves about a wave per SIMD, a channel's states are shared by R / 4 lanes (16x256x100: 21 us
+// with one lane a channel, 15; 1x1024x256: 25 and 18; 64x1024x100, which has twice as many waves: 74 and 96), and a sequence
+// that is short enough is not split at all (64x60x100: in one pass 12, in segments 13; 64x96x100: 17 and 16.5).
+constexpr long kMaxSegments = 256, kSplitFrom = 40, kJoinFrom = 24, kShareBelow = 64, kShareTiles = 6144, kSplitWaves = 2048;
 
 ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
     ScanPlan pl = {};
@@ -1214,9 +1226,9 @@ ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
     long S = 1;
     pl.P = 1;
     if (waves > 0 && waves < 512) {
-        if (forward && a->T < kShareBelow && a->N > 4) pl.P = padded_states(a->N) / 4;
-        else if (a->T >= kSplitFrom) {
-            S = (kSplitWaves + waves - 1) / waves;
+        if (forward && a->N > 4 && (a->T < kShareBelow || waves * tiles <= kShareTiles)) pl.P = padded_states(a->N) / 4;
+        if (a->T >= (pl.P > 1 ? kShareBelow : kSplitFrom)) {
+            S = (kSplitWaves + waves * pl.P - 1) / (waves * pl.P);
             if (S > tiles / 2) S = tiles / 2;
             if (S > kMaxSegments) S = kMaxSegments;
         }
@@ -1332,18 +1344,23 @@ extern "C" int vsv_ssm_scan(const vsv_ssm_desc* a, void* ws, size_t ws_bytes, vo
     return by_dtype(a->dtype, "vsv_ssm_scan", [&](auto t) { return by_states(a->N, [&](auto r) {
         using T = decltype(t);
         constexpr int R = decltype(r)::value;
-        if (pl.S > 1) {
-            hipLaunchKernelGGL((ssm_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
-            if (int rc = op_launch_check("ssm_ends_kernel")) return rc;
-            if (int rc = join_segments<R>(a, pl, a->state_in, false, E, sd, (hipStream_t)stream)) return rc;
-        }
         if constexpr (R > 4) {
             if (pl.P > 1) {
                 constexpr int P = R / 4, kCh = 64 / P;
                 const long groups = a->B * a->G * ((a->D / a->G + kCh - 1) / kCh);
-                hipLaunchKernelGGL((ssm_shared_kernel<T, R, P>), dim3((unsigned)groups), dim3(64), 0, (hipStream_t)stream, *a, pl);
+                if (pl.S > 1) {
+                    hipLaunchKernelGGL((ssm_shared_kernel<T, R, P, true>), dim3((unsigned)(groups * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+                    if (int rc = op_launch_check("ssm_shared_kernel")) return rc;
+                    if (int rc = join_segments<R>(a, pl, a->state_in, false, E, sd, (hipStream_t)stream)) return rc;
+                }
+                hipLaunchKernelGGL((ssm_shared_kernel<T, R, P, false>), dim3((unsigned)(groups * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
                 return op_launch_check("ssm_shared_kernel");
             }
+        }
+        if (pl.S > 1) {
+            hipLaunchKernelGGL((ssm_ends_kernel<T, R>), dim3((unsigned)(waves * (pl.S - 1))), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
+            if (int rc = op_launch_check("ssm_ends_kernel")) return rc;
+            if (int rc = join_segments<R>(a, pl, a->state_in, false, E, sd, (hipStream_t)stream)) return rc;
         }
         hipLaunchKernelGGL((ssm_scan_kernel<T, R>), dim3((unsigned)(waves * pl.S)), dim3(64), 0, (hipStream_t)stream, *a, pl, E, sd);
         return op_launch_check("ssm_scan_kernel");
