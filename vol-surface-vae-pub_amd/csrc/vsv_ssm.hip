@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
 // operations, 24 cycles of a SIMD per 64 channels, against 8 bytes of traffic per channel and step in 16 bits.  Bound by
 // the vector units: 1x16384x2048 bf16 takes 261 us in all, of which the issue of its vector instructions is 227.
 //   A lane owns a channel and its N states (padded to R) in registers (or four of them), a wave 64 channels of one group (or
-// 256 / R), which share b_t and c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are computed; the activations are
-// taken for a tile at a time.
+// 256 / R), which share b_t and c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are
+// computed; the activations are taken for a tile at a time.
 //   A wave runs along time alone, so where sequences and channels make fewer waves than the chip has SIMDs the time axis is
 // split (scan_plan).  A first pass gives every segment's state from zero and its sum of delta; the state in front of a
 // segment then follows from exp(a sum delta), one step per earlier segment: at the start of the second pass or, of many

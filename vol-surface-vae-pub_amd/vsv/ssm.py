@@ -25,15 +25,12 @@ from . import lib as _lib
 from . import native as _native
 
 
-def _call(name, named, *args):
-    """An entry of the native side.  What its signature cannot take is not a tensor where one is wanted: named says which."""
-    try:
-        return getattr(_native.load(), name)(*args)
-    except TypeError:
-        for k, t in named.items():
-            if not isinstance(t, torch.Tensor) and not (t is None and k not in ("x", "weight", "dt", "a", "b", "c", "state")):
-                raise ValueError(f"{name}: {k} must be a tensor, not {t!r}") from None
-        raise
+def _not_a_tensor(name, error, named):
+    """What the native side's signature could not take, named if it is not a tensor where one is wanted."""
+    for k, t in named.items():
+        if not isinstance(t, torch.Tensor) and not (t is None and k not in ("x", "weight", "dt", "a", "b", "c", "state")):
+            return ValueError(f"{name}: {k} must be a tensor, not {t!r}")
+    return error
 
 
 def short_conv(x, weight, bias=None, *, silu=True, initial_state=None, lengths=None, return_state=False):
@@ -41,15 +38,20 @@ def short_conv(x, weight, bias=None, *, silu=True, initial_state=None, lengths=N
 
     x (B, T, D), weight (D, K) with 1 to 4 taps, bias (D).  initial_state (B, K - 1, D): the inputs before the first (zeros
     without it).  Returns y (B, T, D) [, the last K - 1 inputs (B, K - 1, D) in float32]."""
-    out = _call("short_conv", dict(x=x, weight=weight, bias=bias, initial_state=initial_state, lengths=lengths), x, weight, bias, silu,
-                initial_state, lengths, return_state)
+    try:
+        out = _native.load().short_conv(x, weight, bias, silu, initial_state, lengths, return_state)
+    except TypeError as e:
+        raise _not_a_tensor("short_conv", e, dict(x=x, weight=weight, bias=bias, initial_state=initial_state, lengths=lengths)) from None
     return (out[0], out[1]) if return_state else out[0]
 
 
 def short_conv_step(x, state, weight, bias=None, *, silu=True):
     """short_conv for one new token of every row: x (B, D) -> y (B, D); state (B, K - 1, D), contiguous float32, is updated in
     place.  No gradients.  Bit for bit what short_conv gives for the same inputs."""
-    return _call("short_conv_step", dict(x=x, state=state, weight=weight, bias=bias), x, state, weight, bias, silu)
+    try:
+        return _native.load().short_conv_step(x, state, weight, bias, silu)
+    except TypeError as e:
+        raise _not_a_tensor("short_conv_step", e, dict(x=x, state=state, weight=weight, bias=bias)) from None
 
 
 def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=True, initial_state=None, lengths=None,
@@ -61,16 +63,21 @@ def ssm_scan(x, dt, a, b, c, skip=None, gate=None, *, dt_bias=None, softplus=Tru
     For gradients the states before every eighth step are kept (in float32: N / 2 bytes per element of x, N rounded up to
     4, 8 or 16).  A training step captured into a HIP graph wants parameters without a live eager graph of their own, as any
     captured backward pass of torch's does."""
-    out = _call("ssm_scan", dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, dt_bias=dt_bias, initial_state=initial_state, lengths=lengths),
-                x, dt, a, b, c, skip, gate, dt_bias, softplus, initial_state, lengths, return_state)
+    try:
+        out = _native.load().ssm_scan(x, dt, a, b, c, skip, gate, dt_bias, softplus, initial_state, lengths, return_state)
+    except TypeError as e:
+        raise _not_a_tensor("ssm_scan", e, dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, dt_bias=dt_bias,
+                                                initial_state=initial_state, lengths=lengths)) from None
     return (out[0], out[1]) if return_state else out[0]
 
 
 def ssm_step(x, dt, a, b, c, skip=None, gate=None, *, state, dt_bias=None, softplus=True):
     """ssm_scan for one new token of every row: x, dt [, gate] (B, D), b, c (B, [G,] N) -> y (B, D); state (B, D, N),
     contiguous float32, is updated in place.  No gradients."""
-    return _call("ssm_step", dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, state=state, dt_bias=dt_bias),
-                 x, dt, a, b, c, skip, gate, state, dt_bias, softplus)
+    try:
+        return _native.load().ssm_step(x, dt, a, b, c, skip, gate, state, dt_bias, softplus)
+    except TypeError as e:
+        raise _not_a_tensor("ssm_step", e, dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, state=state, dt_bias=dt_bias)) from None
 
 
 # ---- the memory they make up -------------------------------------------------------------------------------------
