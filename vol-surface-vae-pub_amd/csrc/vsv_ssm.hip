@@ -27,9 +27,9 @@ __device__ inline float conv_pre(const float (&w)[K], const float (&x)[K], float
 }
 __device__ inline float conv_silu(float s) {
     constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f, kLn2 = 0.693147182f;       // log2 e, what it is rounded by, 1 / log2 e
-    const float x = __builtin_amdgcn_fmed3f(-s, -100.0f, 100.0f), t = x * kHi;
+    const float x = __builtin_amdgcn_fmed3f(-s, -100.0f, 88.0f), t = x * kHi;
     const float e = exp2_fast(t) * __builtin_fmaf(__builtin_fmaf(x, kLo, __builtin_fmaf(x, kHi, -t)), kLn2, 1.0f);
-    const float y = __builtin_fminf(1.0f + e, 3e38f), r = __builtin_amdgcn_rcpf(y);
+    const float y = 1.0f + e, r = __builtin_amdgcn_rcpf(y);                // (e^88 is the largest that leaves it finite)
     return s * __builtin_fmaf(__builtin_fmaf(-y, r, 1.0f), r, r);
 }
 
@@ -50,10 +50,9 @@ template <typename T, int K, int VEC, int kRows> struct ConvRows {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) out[v] = t < 0 && st ? st[(t + K - 1) * D + v] : 0.0f;
     }
-    __device__ inline void fetch(long t) {                                 // rows t .. t + kRows - 1; behind the last: the last
-        if (len == 0) return;
+    __device__ inline void fetch(const T* at) {                            // kRows rows from here on
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(x + (t + u < len ? t + u : len - 1) * ts);
+        for (int u = 0; u < kRows; ++u) raw[u] = *reinterpret_cast<const Pack<T, VEC>*>(at + u * ts);
     }
     __device__ inline void take(int u, float (&out)[VEC]) const {
 #pragma unroll
@@ -70,7 +69,9 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
     T* y = (T*)a.y + b * a.T * a.D + d0;
     ConvRows<T, K, VEC, kRows> in(a, b, d0);
     float w[VEC][K], bias[VEC], xs[K - 1 + kRows][VEC];
-    if (t0 < in.len) in.fetch(t0);
+    const long lim = t1 < in.len ? t1 : in.len;                           // rows from here on to t1 are padding
+    const T* px = in.x + t0 * in.ts;
+    if (t0 + kRows <= lim) in.fetch(px);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) in.row(t0 - K + 1 + k, xs[k]);
 #pragma unroll
@@ -79,34 +80,44 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
 #pragma unroll
         for (int k = 0; k < K; ++k) w[v][k] = a.w[(d0 + v) * K + k];
     }
-    for (long t = t0; t < t1; t += kRows) {
+    auto put = [&](int u, T* to) {
+        float out[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float win[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) win[k] = xs[u + k][v];
+            out[v] = conv_pre<K>(w[v], win, bias[v]);
+        }
+        if (a.silu) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) out[v] = conv_silu(out[v]);
+        }
+        store_vec<T, VEC>(to, out);
+    };
+    long t = t0;
+    y += t0 * a.D;
+    for (; t + kRows <= lim; t += kRows) {
 #pragma unroll
         for (int u = 0; u < kRows; ++u) in.take(u, xs[K - 1 + u]);
-        if (t + kRows < t1 && t + kRows < in.len) in.fetch(t + kRows);
+        if (t + 2 * kRows <= lim) { px += kRows * in.ts; in.fetch(px); }
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            if (t + u >= t1) break;
-            float out[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float win[K];
-#pragma unroll
-                for (int k = 0; k < K; ++k) win[k] = xs[u + k][v];
-                out[v] = conv_pre<K>(w[v], win, bias[v]);
-            }
-            if (a.silu) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) out[v] = conv_silu(out[v]);
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) out[v] = t + u < in.len ? out[v] : 0.0f;
-            store_vec<T, VEC>(y + (t + u) * a.D, out);
-        }
+        for (int u = 0; u < kRows; ++u, y += a.D) put(u, y);
 #pragma unroll
         for (int k = 0; k < K - 1; ++k)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) xs[k][v] = xs[k + kRows][v];
     }
+    for (; t < lim; ++t, y += a.D) {
+        in.row(t, xs[K - 1]);
+        put(0, y);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) xs[k][v] = xs[k + 1][v];
+    }
+    const float zeros[VEC] = {};
+    for (; t < t1; ++t, y += a.D) store_vec<T, VEC>(y, zeros);
     if (a.state_out && ch == 0) {
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
@@ -133,13 +144,15 @@ __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_con
     const float* dso = g.d_state_out ? g.d_state_out + b * (K - 1) * a.D + d0 : nullptr;
     ConvRows<T, K, VEC, kRows> in(a, b, d0);
     Pack<T, VEC> dyr[kRows];
-    auto fetch = [&](long t) {
-        in.fetch(t);
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) dyr[u] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (t + u < in.len ? t + u : in.len - 1) * g.dy_ts);
-    };
     float w[K][VEC], bias[VEC], xs[K - 1 + kRows][VEC], ds[K - 1 + kRows][VEC], dw[K][VEC], db[VEC];
-    if (t0 < in.len) fetch(t0);
+    const long lim = t1 < in.len ? t1 : in.len;
+    const T *px = in.x + t0 * in.ts, *pdy = dy + t0 * g.dy_ts;
+    auto fetch = [&] {
+        in.fetch(px);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) dyr[u] = *reinterpret_cast<const Pack<T, VEC>*>(pdy + u * g.dy_ts);
+    };
+    if (t0 + kRows <= lim) fetch();
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         in.row(t0 - K + 1 + k, xs[k]);
@@ -153,8 +166,47 @@ __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_con
 #pragma unroll
         for (int k = 0; k < K; ++k) { w[k][v] = a.w[(d0 + v) * K + k]; dw[k][v] = 0.0f; }
     }
+    auto slope = [&](int u, int v, float d) {                             // dy act'(pre) at the window that ends in xs[K - 1 + u]
+        if (!a.silu) return d;
+        float s = bias[v];
+#pragma unroll
+        for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], xs[u + k][v], s);
+        const float sg = sigmoid_f(s);
+        return d * sg * __builtin_fmaf(s, 1.0f - sg, 1.0f);
+    };
+    auto weigh = [&](int u) {                                             // a row's share of dw and db
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float d = ds[K - 1 + u][v];
+            db[v] += d;
+#pragma unroll
+            for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d, xs[u + k][v], dw[k][v]);
+        }
+    };
+    auto back = [&](int u, float (&o)[VEC]) {                             // dx of the row K - 1 in front: ds[to + K-1-k] is ds[u + K-1-k] here
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            o[v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[k][v], ds[u + K - 1 - k][v], o[v]);
+        }
+    };
+    auto shift = [&](int rows) {
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) { xs[k][v] = xs[k + rows][v]; ds[k][v] = ds[k + rows][v]; }
+    };
     const long lo = ch == 0 ? -(K - 1) : t0, end = t1 + K - 1;            // (chunk 0 also returns the state's gradient)
-    for (long t = t0; t < end; t += kRows) {
+    auto give = [&](long to, const float (&o)[VEC]) {
+        if (to >= 0) store_vec<T, VEC>(dx + to * a.D, o);
+        else if (g.d_state_in) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) g.d_state_in[(b * (K - 1) + to + K - 1) * a.D + d0 + v] = o[v];
+        }
+    };
+    long t = t0;
+    for (; t + kRows <= lim; t += kRows) {                                // rows of the chunk, none of them padding
         float dyv[kRows][VEC];
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
@@ -162,52 +214,34 @@ __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_con
 #pragma unroll
             for (int v = 0; v < VEC; ++v) dyv[u][v] = to_f(dyr[u].v[v]);
         }
-        if (t + kRows < end && t + kRows < in.len) fetch(t + kRows);
+        if (t + 2 * kRows <= lim) { px += kRows * in.ts; pdy += kRows * g.dy_ts; fetch(); }
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float d = dyv[u][v];
-                if (a.silu) {
-                    float s = bias[v];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], xs[u + k][v], s);
-                    const float sg = sigmoid_f(s);
-                    d *= sg * __builtin_fmaf(s, 1.0f - sg, 1.0f);
-                }
-                if (t + u >= in.len) d = 0.0f;
-                ds[K - 1 + u][v] = d;
-                if (t + u < t1 && t + u < in.len) {
-                    db[v] += d;
-#pragma unroll
-                    for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d, xs[u + k][v], dw[k][v]);
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            const long to = t + u - (K - 1);                              // dx of this row: ds[to + K-1-k] is ds[u + K-1-k] here
-            if (to < lo || to >= t1) continue;
+            for (int v = 0; v < VEC; ++v) ds[K - 1 + u][v] = slope(u, v, dyv[u][v]);
+            weigh(u);
             float o[VEC];
-            const long j = to - (in.len - (K - 1));                       // the row of state_out that xs[to] is, if any
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float s = 0.0f;
-#pragma unroll
-                for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][v], ds[u + K - 1 - k][v], s);
-                if (dso && j >= 0 && j < K - 1) s += dso[j * a.D + v];
-                o[v] = s;
-            }
-            if (to >= 0) store_vec<T, VEC>(dx + to * a.D, o);
-            else if (g.d_state_in) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) g.d_state_in[(b * (K - 1) + to + K - 1) * a.D + d0 + v] = o[v];
-            }
+            back(u, o);
+            const long to = t + u - (K - 1);
+            if (to >= lo) give(to, o);
         }
+        shift(kRows);
+    }
+    for (; t < end; ++t) {                                                // what is left of it, and the K - 1 rows behind it
+        in.row(t, xs[K - 1]);
+        float dyv[VEC] = {}, o[VEC];
+        if (t < in.len) load_vec<T, VEC>(dy + t * g.dy_ts, dyv);
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k)
+        for (int v = 0; v < VEC; ++v) ds[K - 1][v] = t < in.len ? slope(0, v, dyv[v]) : 0.0f;
+        if (t < lim) weigh(0);
+        back(0, o);
+        const long to = t - (K - 1), jj = to - (in.len - (K - 1));        // (the row of state_out that xs[to] is, if any)
+        if (dso && jj >= 0 && jj < K - 1) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) { xs[k][v] = xs[k + kRows][v]; ds[k][v] = ds[k + kRows][v]; }
+            for (int v = 0; v < VEC; ++v) o[v] += dso[jj * a.D + v];
+        }
+        if (to >= lo && to < t1) give(to, o);
+        shift(1);
     }
     float* p = part + (b * n_chunk + ch) * (K + 1) * a.D + d0;
 #pragma unroll
