@@ -34,7 +34,7 @@ __device__ inline float conv_silu(float s) {
 }
 
 // pre[t,d] = bias[d] + sum_k w[d,k] xs[t-K+1+k, d],  y = silu(pre) or pre; xs is x, continued into state_in before t = 0.
-// One read of x and one write of y (2K flops an element): bound by memory (8x2048x4096 bf16: 66 us, 4.0 TB/s).  A thread owns VEC
+// One read of x and one write of y (2K flops an element): bound by memory (8x2048x4096 bf16: 61 us, 4.4 TB/s).  A thread owns VEC
 // neighbouring channels and a chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it
 // works on kRows rows at a time, with the next ones under way.
 template <typename T, int K, int VEC, int kRows> struct ConvRows {
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
 
 // ds = dy act'(pre) (pre computed again from x), dx[t] = sum_k w[k] ds[t+K-1-k], dw[k] = sum_t ds[t] xs[t-K+1+k],
 // dbias = sum_t ds.  The same chunks; a chunk reads K-1 rows beyond each end, its sums over time go to `part`
-// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.  8x2048x4096 bf16: 105 us, 3.8 TB/s.
+// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.  8x2048x4096 bf16: 92 us, 4.4 TB/s.
 template <typename T, int K, int VEC, int kRows>
 __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_conv_desc a, const vsv_short_conv_grads g, long chunk, long n_chunk,
                                                              long n_vec, float* __restrict__ part) {
@@ -1184,17 +1184,15 @@ bool conv_words(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g, siz
     if (g) ok = ok && g->dy_bs % v == 0 && g->dy_ts % v == 0 && aligned(g->dy, v * size) && aligned(g->dx, v * size);
     return ok;
 }
-// Channels per thread: four where the rows allow it; backward eight in 16 bits (two rows under way instead of four fit the
-// registers: 8x2048x4096 bf16 108 us for 131; forward they are slower, 80 for 67).
+// Channels per thread: four where the rows allow it (eight in 16 bits: forward 80 us for 67, backward the same 92 us).
 int conv_vec(const vsv_short_conv_desc* a, const vsv_short_conv_grads* g) {
     const size_t size = a->dtype == VSV_F32 ? 4 : 2;
-    if (g && size == 2 && conv_words(a, g, size, 8)) return 8;
     return conv_words(a, g, size, 4) ? 4 : 1;
 }
 
 // Time steps per thread: the longer, the less is read twice and the fewer sums are left over, as long as the threads fill the
-// chip.  Forward eight waves for every SIMD (8x2048x4096 bf16: two 69 us, eight 66, sixteen 68); backward, where a chunk leaves
-// K + 1 sums per channel, two (108 us and 5 for the sums; one 157, four 120 and 11).
+// chip.  Forward eight waves for every SIMD (8x2048x4096 bf16: four and eight 61 us); backward, where a chunk leaves K + 1 sums
+// per channel, two (92 us and 4 for the sums; one 105 and 5, four 100 and 7).
 constexpr long kConvFill = 524288, kConvBwdFill = 131072;
 long conv_chunk(const vsv_short_conv_desc* a, long fill, long vec) {
     const long rows = a->B * (a->D / vec);
@@ -1205,8 +1203,7 @@ long conv_chunk(const vsv_short_conv_desc* a, long fill, long vec) {
 long conv_chunks(const vsv_short_conv_desc* a, long chunk) { return a->T > 0 ? (a->T + chunk - 1) / chunk : 1; }
 // The backward pass's chunk goes by the sizes alone, so that its workspace does too.
 long conv_bwd_chunk(const vsv_short_conv_desc* a) {
-    const bool half = a->dtype != VSV_F32;
-    return conv_chunk(a, kConvBwdFill, half && a->D % 8 == 0 ? 8 : a->D % 4 == 0 ? 4 : 1);
+    return conv_chunk(a, kConvBwdFill, a->D % 4 == 0 ? 4 : 1);
 }
 
 template <typename F> int by_taps(int K, F&& f) {
@@ -1323,12 +1320,6 @@ extern "C" int vsv_short_conv_backward(const vsv_short_conv_desc* a, const vsv_s
         const int rc = by_dtype(a->dtype, "vsv_short_conv_backward", [&](auto t) { return by_taps(a->K, [&](auto k) {
             using T = decltype(t);
             constexpr int K = decltype(k)::value;
-            if constexpr (sizeof(T) == 2) {
-                if (vec == 8) {
-                    hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 8, 2>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, chunk, nc, nv, (float*)ws);
-                    return op_launch_check("short_conv_bwd_kernel");
-                }
-            }
             if (vec == 4) hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 4, 4>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, chunk, nc, nv, (float*)ws);
             else hipLaunchKernelGGL((short_conv_bwd_kernel<T, K, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, *a, *g, chunk, nc, nv, (float*)ws);
             return op_launch_check("short_conv_bwd_kernel");
