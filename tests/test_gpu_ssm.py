@@ -527,3 +527,77 @@ def test_step_with_b_and_c_anywhere(N, dtype):
     for y, st in zip(ys, states):
         _scan_check(s, {"y": y[:, None], "state": st})
         assert torch.equal(y, ys[0]) and torch.equal(st, states[0])
+
+
+def test_gradients_past_32_bits():
+    """More than 2^31 elements: two sequences of the same inputs have the same outputs and gradients, wherever they lie."""
+    from vsv.ssm import short_conv, ssm_scan, ssm_step
+    T, D, N = (1 << 20) + 5, 1100, 8
+    r = lambda *shape: torch.randn(*shape, device="cuda").to(torch.bfloat16)
+    x, b, w = r(1, T, D).expand(2, T, D), r(1, T, N).expand(2, T, N), torch.randn(D, 4, device="cuda")
+    a, dy = -torch.rand(D, N, device="cuda") - 0.1, r(1, T, D).expand(2, T, D)
+    for call in (lambda t: short_conv(t, w), lambda t: ssm_scan(t, x[:, :t.shape[1]], a, b[:, :t.shape[1]], b[:, :t.shape[1]], gate=x[:, :t.shape[1]])):
+        leaf = x.detach().requires_grad_(True)
+        y = call(leaf)
+        assert y.numel() > 2**31 and torch.equal(y[0], y[1]) and y[1, -1].abs().sum() > 0
+        g, = torch.autograd.grad(y, leaf, dy)
+        assert torch.equal(g[0], g[1]) and g[1, -1].abs().sum() > 0
+        short = call(x[:, :300])                                              # (the front, computed in another number of segments)
+        assert (short[1] - y[1, :300]).abs().max() <= 2.0 ** -7 * y[1, :300].abs().max()
+        del y, g, leaf, short
+    B, D = 33000, 4096
+    state = torch.zeros(B, D, 16, device="cuda")
+    assert state.numel() > 2**31
+    x, b, a = r(1, D).expand(B, D), r(1, 16).expand(B, 16), -torch.rand(D, 16, device="cuda")
+    y = ssm_step(x, x, a, b, b, state=state)
+    assert torch.equal(y[-1], y[0]) and torch.equal(state[-1], state[0]) and state[-1].abs().sum() > 0
+
+
+def test_tokens_captured_and_replayed():
+    """One token's two steps in a HIP graph: every replay takes the next token and moves the states on, as eager calls do."""
+    from vsv.ssm import short_conv_step, ssm_step
+    s, k = _scan_case(46, 3, 6, 72, 16, 1, "bf16"), _conv_case(47, 3, 6, 72, 4, "bf16")
+
+    def token(x, dt, b, c, gate, conv_state, state):
+        u = short_conv_step(x, conv_state, k["w"], k["bias"])
+        return ssm_step(u, dt, s["a"], b, c, s["skip"], gate, state=state, dt_bias=s["dt_bias"])
+    inputs = [[t[:, i].clone() for t in (k["x"], s["dt"], s["b"], s["c"], s["gate"])] for i in range(6)]
+    want_states = [k["h0"].clone(), s["h0"].clone()]
+    want = [token(*i, *want_states) for i in inputs]
+    held, states = [t.clone() for t in inputs[0]], [k["h0"].clone(), s["h0"].clone()]
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+            out = token(*held, *states)
+    for i, y in zip(inputs, want):
+        for h, t in zip(held, i):
+            h.copy_(t)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)
+        (out.float() @ out.float().t()).sum().item()                          # (eager work in between)
+    assert all(torch.equal(g, w) for g, w in zip(states, want_states))
+
+
+def test_two_threads_at_once():
+    """Calls of two threads on their own streams, forward and backward, give what each gives alone."""
+    import threading
+    cases = [_scan_case(48, 2, 300, 130, 16, 1, "fp32"), _scan_case(49, 3, 90, 100, 8, 1, "bf16")]
+    want = [_scan_run(s) for s in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = _scan_run(cases[i])
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(n for n in got if not torch.equal(got[n], want[i][n]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

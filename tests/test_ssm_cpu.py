@@ -160,6 +160,21 @@ def test_optimizer_refuses_parameters_that_share_memory():
     assert opt.state[p]["step"] == 0
 
 
+def test_optimizer_refuses_other_rules_options():
+    from vsv.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    for bad in (dict(maximize=True), dict(amsgrad=True), dict(decoupled_weight_decay=False)):
+        with pytest.raises(ValueError, match="not built"):
+            AdamW([{"params": [p], **bad}])
+        theirs = torch.optim.AdamW([p]).state_dict()
+        theirs["param_groups"][0].update(bad)
+        with pytest.raises(ValueError, match="not built"):
+            AdamW([p]).load_state_dict(theirs)
+    opt = AdamW([p])
+    opt.load_state_dict(torch.optim.AdamW([p], lr=0.25).state_dict())          # torch's own, of the same rule
+    assert opt.param_groups[0]["lr"] == 0.25
+
+
 def test_c_entries_check_their_arguments():
     from vsv import lib as vlib
     L = vlib.load()

@@ -41,6 +41,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: bad hyper-parameters lr={lr} betas={g['betas']} eps={eps} weight_decay={wd}")
             if g["state_bits"] != self.state_bits:
                 raise ValueError("AdamW: all groups hold their moments in the same number of bits")
+            _check_options(g)
             if len(set(map(id, g["params"]))) < len(g["params"]):
                 raise ValueError("AdamW: a parameter is in its group twice")
             for p in g["params"]:
@@ -108,6 +109,8 @@ class AdamW(torch.optim.Optimizer):
         params = [p for g in self.param_groups for p in g["params"]]
         if any(g.get("state_bits", self.state_bits) != self.state_bits for g in state_dict["param_groups"]):
             raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
+        for g in state_dict["param_groups"]:
+            _check_options(g)
         for i, p in zip(saved, params):
             st = state_dict["state"].get(i)
             if st and set(st) != {"step", *self._layout(p)}:
@@ -120,6 +123,12 @@ class AdamW(torch.optim.Optimizer):
             if state_dict["state"].get(i):
                 self.state[p] = {k: v.detach().to(device=p.device, copy=True).contiguous() if torch.is_tensor(v) else int(v)
                                  for k, v in state_dict["state"][i].items()}
+
+
+def _check_options(group):
+    """Options of torch's Adam family that a group, or a state saved by one of them, may carry and this step does not have."""
+    if group.get("amsgrad") or group.get("maximize") or (group.get("decoupled_weight_decay") is False and group["weight_decay"]):
+        raise ValueError("AdamW: amsgrad, maximize and coupled weight decay are not built")
 
 
 def _check_param(p):
