@@ -650,7 +650,8 @@ int vsv_ssm_step(const vsv_ssm_desc *a, void *stream);
 
 /* ---- AdamW over many tensors, moments in 32 or 8 bits ------------------------------------------------------
  * The optimizer step of vsv_adamw_step for tensors with gradients of their own, in float32, bfloat16 or float16 (`dtype`
- * of p and g).  `tensors` is a HOST array; its contents travel in the launches' arguments (60 tensors each).
+ * of p and g).  `tensors` is a HOST array; its contents travel in the launches' arguments (60 tensors each).  No two entries may
+ * share memory that is written.
  * bits = 32: m, v float32.  bits = 8: m int8, v uint8 codes with a float32 scale of each per VSV_ADAMW_BLOCK elements
  * (m = sign s (k/127)^2, v = s (k/255)^4, to float32).  All state starts as zeros; step = the count after this step (>= 1).
  * vsv_adamw_read8: p and g of an entry are two float32 outputs and receive the values m and v stand for. */
