@@ -337,3 +337,32 @@ def test_model_train_step_takes_it(bits):
     assert b.abs().max() > 1e-3
     assert ((a - b).norm() / a.norm()).item() <= (2e-3 if bits == 32 else 0.1)
     assert abs(lw[2] - lg[2]) <= 1e-2 * abs(lw[2])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_first_step_under_capture_leaves_no_state(bits):
+    """Refused before the moments are made (their zeros would only be recorded): the eager step behind it starts from zero moments, as
+    a new optimizer's does, and replays of the graph leave them alone."""
+    from vsv.optim import AdamW
+    g = torch.Generator().manual_seed(6)
+    p = torch.nn.Parameter(torch.randn(1000, generator=g).cuda())
+    q = torch.nn.Parameter(p.detach().clone())
+    opt, other = AdamW([p], state_bits=bits, **HYPER), AdamW([q], state_bits=bits, **HYPER)
+    p.grad = torch.randn(1000, generator=g).cuda()
+    q.grad = p.grad.clone()
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+    assert len(opt.state) == 0
+    for turn in range(3):
+        graph.replay()
+        opt.step(); other.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q), turn
+        assert all(torch.equal(a, b) for one, two in zip(opt.moments(), other.moments()) for a, b in zip(one, two)), turn
+    assert x[0].item() == 6

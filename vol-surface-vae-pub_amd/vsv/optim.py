@@ -68,6 +68,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # (before any state is made: under capture its zeros would only be recorded)
+        for index in {p.get_device() for group in self.param_groups for p in group["params"] if p.grad is not None}:
+            if index >= 0 and _capturing(index):
+                raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
         state, calls, states = self.state, [], []
         wide = self.state_bits == 32
         for group in self.param_groups:
@@ -85,8 +89,6 @@ class AdamW(torch.optim.Optimizer):
                               float(group["lr"]), float(b1), float(b2), float(group["eps"]), float(group["weight_decay"]), step + 1))
                 states += sts
         if calls:
-            if calls[0][0][0].is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
             _native.load().adamw_step(self.state_bits, calls)              # (checks everything before it launches anything)
             for st in states:
                 st["step"] += 1
@@ -123,6 +125,11 @@ class AdamW(torch.optim.Optimizer):
             if state_dict["state"].get(i):
                 self.state[p] = {k: v.detach().to(device=p.device, copy=True).contiguous() if torch.is_tensor(v) else int(v)
                                  for k, v in state_dict["state"][i].items()}
+
+
+def _capturing(index):
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _check_options(group):
