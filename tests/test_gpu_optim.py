@@ -366,3 +366,29 @@ def test_a_first_step_under_capture_leaves_no_state(bits):
         assert torch.equal(p, q), turn
         assert all(torch.equal(a, b) for one, two in zip(opt.moments(), other.moments()) for a, b in zip(one, two)), turn
     assert x[0].item() == 6
+
+
+def test_continues_a_checkpoint_of_torchs():
+    """State of a torch.optim.AdamW after three steps, loaded, then three more of either: the parameters agree to the rounding of
+    test_32_bits' bound (3 s + 1 half steps on the moments, s = 6, 8 on the update, 3 and one more a step on the parameter), twice."""
+    from vsv.optim import AdamW
+    g = torch.Generator().manual_seed(8)
+    ps = [torch.nn.Parameter(torch.randn(s, generator=g).cuda()) for s in SIZES]
+    theirs = torch.optim.AdamW(ps, **HYPER)
+    for _ in range(3):
+        _grads(ps, g)
+        theirs.step()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt = AdamW(qs)
+    opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["weight_decay"] == HYPER["weight_decay"]
+    for t in range(4, 7):
+        _grads(ps, g)
+        for p, q in zip(ps, qs):
+            q.grad = p.grad.clone()
+        theirs.step(); opt.step()
+        for p, q in zip(ps, qs):
+            st = theirs.state[p]
+            assert opt.state[q]["step"] == t == int(st["step"])
+            size = p.detach().abs() + HYPER["lr"] * 10                       # (|m| / sqrt(v) of a few equal shares is below 10)
+            assert ((p - q).detach().abs() <= 2.0 ** -24 * 2 * (4 * t + 30) * size).all()

@@ -175,6 +175,38 @@ def test_optimizer_refuses_other_rules_options():
     assert opt.param_groups[0]["lr"] == 0.25
 
 
+def _stepped(make, sizes=(4, 9, 300), steps=3):
+    """Parameters of their own and torch's optimizer after some steps of theirs."""
+    g = torch.Generator().manual_seed(5)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=g)) for n in sizes]
+    opt = make(ps)
+    for _ in range(steps):
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g)
+        opt.step()
+    return ps, opt
+
+
+def test_state_of_a_stepped_torch_optimizer(monkeypatch):
+    """Its step counts are tensors: they become numbers, so that the parameters stay together in one call."""
+    from vsv import native
+    from vsv.optim import AdamW
+    ps, theirs = _stepped(lambda q: torch.optim.AdamW(q, lr=1e-2))
+    opt = AdamW(ps)
+    opt.load_state_dict(theirs.state_dict())
+    assert [type(opt.state[p]["step"]) for p in ps] == [int] * 3 and [opt.state[p]["step"] for p in ps] == [3] * 3
+    assert all(torch.equal(opt.state[p][k], theirs.state[p][k]) and opt.state[p][k].data_ptr() != theirs.state[p][k].data_ptr()
+               for p in ps for k in ("exp_avg", "exp_avg_sq"))
+    made = []
+
+    class Native:
+        def adamw_step(self, bits, calls):
+            made.extend((len(c[0]), c[-1]) for c in calls)
+    monkeypatch.setattr(native, "load", Native)
+    opt.step()
+    assert made == [(3, 4)] and [opt.state[p]["step"] for p in ps] == [4] * 3
+
+
 def test_c_entries_check_their_arguments():
     from vsv import lib as vlib
     L = vlib.load()

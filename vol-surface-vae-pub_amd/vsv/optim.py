@@ -123,7 +123,8 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict(state_dict)
         for i, p in zip(saved, params):
             if state_dict["state"].get(i):
-                self.state[p] = {k: v.detach().to(device=p.device, copy=True).contiguous() if torch.is_tensor(v) else int(v)
+                # (torch's own optimizers keep the step count in a tensor: here it groups the parameters, and is a launch argument)
+                self.state[p] = {k: int(v) if k == "step" else v.detach().to(device=p.device, copy=True).contiguous()
                                  for k, v in state_dict["state"][i].items()}
 
 
