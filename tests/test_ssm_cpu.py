@@ -207,6 +207,35 @@ def test_state_of_a_stepped_torch_optimizer(monkeypatch):
     assert made == [(3, 4)] and [opt.state[p]["step"] for p in ps] == [4] * 3
 
 
+def test_hooks_of_load_state_dict():
+    """A pre-hook's dictionary is the one that is taken (and checked), a post-hook sees the state as it will be, and its changes stay."""
+    from vsv.optim import AdamW
+    ps, theirs = _stepped(lambda q: torch.optim.AdamW(q, lr=1e-2))
+    ps[0].data = ps[0].data.bfloat16()                                      # (its moments stay float32)
+    opt = AdamW(ps)
+    seen = []
+
+    def double(_, d):
+        return {**d, "state": {i: {**st, "exp_avg": 2 * st["exp_avg"]} for i, st in d["state"].items()}}
+
+    def after(o):
+        seen.extend((o.state[p]["step"], o.state[p]["exp_avg"].dtype) for p in ps)
+        o.state[ps[1]]["exp_avg"].zero_()
+    handles = [opt.register_load_state_dict_pre_hook(double), opt.register_load_state_dict_post_hook(after)]
+    saved = theirs.state_dict()
+    opt.load_state_dict(saved)
+    assert seen == [(3, torch.float32)] * 3
+    assert all(torch.equal(opt.state[p]["exp_avg"], k * theirs.state[p]["exp_avg"]) for p, k in zip(ps, (2, 0, 2)))
+    assert all(torch.equal(opt.state[p]["exp_avg_sq"], theirs.state[p]["exp_avg_sq"]) for p in ps)
+    for h in handles:
+        h.remove()
+    opt.load_state_dict(saved)                                              # (nothing of the first call is left)
+    assert torch.equal(opt.state[ps[1]]["exp_avg"], theirs.state[ps[1]]["exp_avg"])
+    opt.register_load_state_dict_pre_hook(lambda _, d: {**d, "state": {0: {**d["state"][0], "exp_avg": torch.zeros(5)}}})
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.load_state_dict(saved)
+
+
 def test_c_entries_check_their_arguments():
     from vsv import lib as vlib
     L = vlib.load()

@@ -106,26 +106,39 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments keep their own types (torch's casts floating state to the parameter's), and nothing that
-        does not fit the parameters is taken."""
+        does not fit the parameters is taken.  Hooks see and change what they do of torch's."""
+        given = []
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, d: given.append(self._fitting(d))),      # (behind every other)
+                 self.register_load_state_dict_post_hook(lambda _: self._take(given[0]), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _fitting(self, state_dict):
+        """[(parameter, its saved state or None)], refused where it does not fit."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         if any(g.get("state_bits", self.state_bits) != self.state_bits for g in state_dict["param_groups"]):
             raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
         for g in state_dict["param_groups"]:
             _check_options(g)
-        for i, p in zip(saved, params):
-            st = state_dict["state"].get(i)
+        rows = [(p, state_dict["state"].get(i)) for i, p in zip(saved, params)]
+        for p, st in rows:
             if st and set(st) != {"step", *self._layout(p)}:
                 raise ValueError(f"AdamW: the saved moments are not held in {self.state_bits} bits")
             for k, (shape, dtype) in self._layout(p).items() if st else ():
                 if tuple(st[k].shape) != tuple(shape) or st[k].dtype != dtype:
                     raise ValueError(f"AdamW: saved {k} is {st[k].dtype} {tuple(st[k].shape)}, not {dtype} {tuple(shape)}")
-        super().load_state_dict(state_dict)
-        for i, p in zip(saved, params):
-            if state_dict["state"].get(i):
+        return rows
+
+    def _take(self, rows):
+        for p, st in rows:
+            if st:
                 # (torch's own optimizers keep the step count in a tensor: here it groups the parameters, and is a launch argument)
                 self.state[p] = {k: int(v) if k == "step" else v.detach().to(device=p.device, copy=True).contiguous()
-                                 for k, v in state_dict["state"][i].items()}
+                                 for k, v in st.items()}
 
 
 def _capturing(index):
