@@ -136,6 +136,26 @@ def test_optimizer_refuses():
         AdamW([p], state_bits=8).load_state_dict({"state": {0: {"step": 1, "exp_avg": torch.zeros(4, 3)}}, "param_groups": opt.state_dict()["param_groups"]})
 
 
+def test_optimizer_refuses_negative_views():
+    """Contiguous tensors whose memory holds the values' opposites: read raw, a step would go the wrong way."""
+    from vsv.optim import AdamW
+    neg = torch._neg_view(torch.ones(4))
+    assert neg.is_contiguous() and neg.is_neg()
+    with pytest.raises(ValueError, match="negative"):
+        AdamW([torch.nn.Parameter(neg)])
+    p = torch.nn.Parameter(torch.ones(4))
+    opt = AdamW([p])
+    p.data, p.grad = neg, torch.ones(4)
+    with pytest.raises(ValueError, match="negative"):
+        opt.step()
+    p.data = torch.ones(4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        opt.step()
+    opt.state[p]["exp_avg"] = torch._neg_view(torch.zeros(4))
+    with pytest.raises(ValueError, match="state was made"):
+        opt.step()
+
+
 def test_optimizer_refuses_parameters_that_share_memory():
     from vsv.optim import AdamW
     flat = torch.zeros(24)

@@ -380,7 +380,7 @@ using Tensors = std::vector<Tensor>;
 using AdamwCall = std::tuple<Tensors, Tensors, Tensors, Tensors, Tensors, Tensors, double, double, double, double, double, int64_t>;
 
 void state_fits(const Tensor& p, const Tensor& t, at::ScalarType type, int64_t n) {
-    TORCH_CHECK_VALUE(t.numel() == n && t.scalar_type() == type && t.device() == p.device() && t.is_contiguous(),
+    TORCH_CHECK_VALUE(t.numel() == n && t.scalar_type() == type && t.device() == p.device() && t.is_contiguous() && !t.is_neg(),
                       "AdamW: a parameter has changed its shape or device since its state was made");
 }
 
@@ -398,7 +398,7 @@ void adamw_step(int bits, std::vector<AdamwCall> calls) {
                           " betas=(", b1, ", ", b2, ") eps=", eps, " weight_decay=", wd);
         for (size_t i = 0; i < p.size(); ++i) {
             TORCH_CHECK_VALUE(type_code(p[i]) >= 0, "AdamW: parameters must be float32, bfloat16 or float16, not ", p[i].scalar_type());
-            TORCH_CHECK_VALUE(p[i].is_contiguous(), "AdamW: parameters must be contiguous");
+            TORCH_CHECK_VALUE(p[i].is_contiguous() && !p[i].is_neg(), "AdamW: parameters must be contiguous, and no negative views");
             TORCH_CHECK_VALUE(g[i].layout() == at::kStrided && g[i].scalar_type() == p[i].scalar_type() && g[i].device() == p[i].device() &&
                                   g[i].sizes() == p[i].sizes(), "AdamW: a gradient needs its parameter's type, device and shape, and no sparse layout");
             const uintptr_t at = (uintptr_t)p[i].data_ptr();

@@ -155,5 +155,5 @@ def _check_options(group):
 def _check_param(p):
     if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError(f"AdamW: parameters must be float32, bfloat16 or float16, not {p.dtype}")
-    if not p.is_contiguous():
-        raise ValueError("AdamW: parameters must be contiguous")
+    if not p.is_contiguous() or p.is_neg():                                # (a negative view's memory holds the values' opposites)
+        raise ValueError("AdamW: parameters must be contiguous, and no negative views")
