@@ -601,3 +601,23 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_forward_mode_is_refused():
+    """Forward, in either mode, and backward from an output's gradient that carries a tangent; without one, a dual level changes nothing."""
+    import torch.autograd.forward_ad as fwd
+    from vsv.ssm import short_conv, ssm_scan
+    s, k = _scan_case(50, 2, 9, 8, 4, 1, "fp32"), _conv_case(51, 2, 9, 8, 4, "fp32")
+    calls = (lambda x: ssm_scan(x, s["dt"], s["a"], s["b"], s["c"]), lambda x: short_conv(x, k["w"]))
+    with fwd.dual_level():
+        for call in calls:
+            want = call(s["x"])
+            for on in (True, False):
+                with torch.set_grad_enabled(on), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(fwd.make_dual(s["x"], torch.ones_like(s["x"])))
+            leaf = s["x"].clone().requires_grad_(True)
+            y = call(leaf)
+            assert torch.equal(y, want)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, fwd.make_dual(s["dy"], torch.ones_like(s["dy"])), retain_graph=True)
+            torch.autograd.grad(y, leaf, s["dy"])

@@ -95,6 +95,25 @@ def test_steps_refuse():
         ssm_step(x, x, a, torch.zeros(2, 4), b, state=torch.zeros(3, 6, 4))
 
 
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """An input with a tangent, whether or not gradients are enabled: the output would have none."""
+    import torch.autograd.forward_ad as fwd
+    from vsv.ssm import short_conv, short_conv_step, ssm_scan, ssm_step
+    t = {**_scan_tensors(), "skip": torch.zeros(6), "gate": torch.zeros(2, 4, 6), "dt_bias": torch.zeros(6), "initial_state": torch.zeros(2, 6, 4)}
+    conv = dict(x=torch.zeros(2, 4, 6), weight=torch.zeros(6, 3), bias=torch.zeros(6), initial_state=torch.zeros(2, 2, 6))
+    step = {k: v[:, 0] if k in ("x", "dt", "b", "c", "gate") else v for k, v in t.items()}
+    step["state"] = step.pop("initial_state")
+    conv_step = dict(x=torch.zeros(2, 6), state=torch.zeros(2, 2, 6), weight=torch.zeros(6, 3), bias=torch.zeros(6))
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        for call, args in ((ssm_scan, t), (short_conv, conv), (ssm_step, step), (short_conv_step, conv_step)):
+            for name, v in args.items():
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(**{**args, name: fwd.make_dual(v, torch.ones_like(v))})
+            with pytest.raises(RuntimeError, match="GPU"):                  # (none: the next refusal)
+                call(**args)
+
+
 def test_no_cpu_fallback():
     from vsv.optim import AdamW
     from vsv.ssm import short_conv, short_conv_step, ssm_scan, ssm_step

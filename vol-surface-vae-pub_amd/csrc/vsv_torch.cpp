@@ -115,6 +115,12 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     return false;
 }
 
+// A tangent would be dropped without a word: what follows looks at requires_grad and at memory alone.
+void no_tangents(const char* what, std::initializer_list<Tensor> ts) {
+    for (const Tensor& t : ts)
+        TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative, and an input carries a tangent");
+}
+
 Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 // (straight from the allocator: through the dispatcher a tensor costs the host twice as much, and a backward pass makes twelve)
@@ -178,6 +184,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
         const Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &h0 = saved[3], &lengths = saved[4];
         Tensor dy = grads[0], dstate = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !dstate.defined()) return variable_list(7);
+        no_tangents("short_conv's backward pass", {dy, dstate});
         Tensor dx, dw, db, dh;
         {
             at::NoGradGuard no_grad;
@@ -214,6 +221,7 @@ variable_list short_conv(const Tensor& x_, const Tensor& weight, const OptTensor
     const Tensor x = seq(what, "x", x_, x_.sizes(), std::nullopt);
     const Tensor w = f32(what, "weight", weight, {D, K}), bias = f32(what, "bias", bias_, {D}), h0 = f32(what, "initial_state", state_, {B, K - 1, D});
     const Tensor lengths = int_lengths(what, lengths_, B);
+    no_tangents(what, {x, w, bias, h0});
     same_gpu(what, x, {w, bias, h0, lengths});
     if (wants_grad({x, w, bias, h0})) return ShortConv::apply(x, w, opt(bias), opt(h0), opt(lengths), silu, want);
     return conv_forward(x, w, bias, h0, lengths, silu, want);
@@ -226,6 +234,7 @@ Tensor short_conv_step(const Tensor& x_, const Tensor& state, const Tensor& weig
     const int64_t B = x_.size(0), D = x_.size(1), K = weight.size(1);
     const Tensor x = seq(what, "x", x_, x_.sizes(), std::nullopt), w = f32(what, "weight", weight, {D, K}), bias = f32(what, "bias", bias_, {D});
     in_place(what, state, {B, K - 1, D});
+    no_tangents(what, {x, w, bias, state});
     same_gpu(what, x, {w, bias, state});
     TORCH_CHECK(!wants_grad({x, w, bias, state}), what, " has no gradient: call it under torch.no_grad()");
     c10::DeviceGuard guard(x.device());
@@ -321,6 +330,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
         const Tensor &h0 = s[8], &lengths = s[9], &saved = s[10];
         Tensor dy = grads[0], dstate = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !dstate.defined()) return variable_list(12);
+        no_tangents("ssm_scan's backward pass", {dy, dstate});
         Tensor dx, ddt, dgate, db, dc, da, dskip, dbias, dh;
         {
             at::NoGradGuard no_grad;
@@ -351,6 +361,7 @@ variable_list ssm_scan(const Tensor& x, const Tensor& dt, const Tensor& a, const
     TORCH_CHECK_VALUE(x.dim() == 3, what, ": x must be a tensor (B, T, D)");
     const ScanArgs r = scan_args(what, x, dt, a, b, c, skip, gate, dt_bias);
     const Tensor h0 = f32(what, "initial_state", state_, {x.size(0), x.size(2), a.size(1)}), lengths = int_lengths(what, lengths_, x.size(0));
+    no_tangents(what, {r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0});
     same_gpu(what, r.x, {r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0, lengths});
     if (wants_grad({r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0}))
         return SsmScan::apply(r.x, r.dt, r.a, r.b, r.c, opt(r.skip), opt(r.gate), opt(r.dt_bias), opt(h0), opt(lengths), softplus, want);
@@ -363,6 +374,7 @@ Tensor ssm_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor
     TORCH_CHECK_VALUE(x.dim() == 2, what, ": x must be a tensor (B, D)");
     const ScanArgs r = scan_args(what, x, dt, a, b, c, skip, gate, dt_bias);
     in_place(what, state, {x.size(0), x.size(1), a.size(1)});
+    no_tangents(what, {r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state});
     same_gpu(what, r.x, {r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state});
     TORCH_CHECK(!wants_grad({r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state}), what, " has no gradient: call it under torch.no_grad()");
     c10::DeviceGuard guard(r.x.device());
