@@ -114,6 +114,21 @@ def test_forward_mode_is_refused(grad):
                 call(**args)
 
 
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+@pytest.mark.parametrize("grad", [True, False])
+def test_tracing_is_refused(grad):
+    """A trace would hold the outputs of the inputs it was made with."""
+    from vsv.ssm import short_conv, short_conv_step, ssm_scan, ssm_step
+    t = _scan_tensors()
+    b = t["b"]
+    with torch.set_grad_enabled(grad):
+        for call, x in ((lambda x: ssm_scan(x, x, t["a"], b, b), t["x"]), (lambda x: short_conv(x, torch.zeros(6, 3)), t["x"]),
+                        (lambda x: ssm_step(x, x, t["a"], b[:, 0], b[:, 0], state=torch.zeros(2, 6, 4)), t["x"][:, 0]),
+                        (lambda x: short_conv_step(x, torch.zeros(2, 2, 6), torch.zeros(6, 3)), t["x"][:, 0])):
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(call, x)
+
+
 def test_no_cpu_fallback():
     from vsv.optim import AdamW
     from vsv.ssm import short_conv, short_conv_step, ssm_scan, ssm_step

@@ -6,6 +6,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -121,6 +122,9 @@ void no_tangents(const char* what, std::initializer_list<Tensor> ts) {
         TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative, and an input carries a tangent");
 }
 
+// A tracer sees none of the calls below: it would keep this call's outputs as constants.
+void not_traced(const char* what) { TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced"); }
+
 Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 // (straight from the allocator: through the dispatcher a tensor costs the host twice as much, and a backward pass makes twelve)
@@ -221,6 +225,7 @@ variable_list short_conv(const Tensor& x_, const Tensor& weight, const OptTensor
     const Tensor x = seq(what, "x", x_, x_.sizes(), std::nullopt);
     const Tensor w = f32(what, "weight", weight, {D, K}), bias = f32(what, "bias", bias_, {D}), h0 = f32(what, "initial_state", state_, {B, K - 1, D});
     const Tensor lengths = int_lengths(what, lengths_, B);
+    not_traced(what);
     no_tangents(what, {x, w, bias, h0});
     same_gpu(what, x, {w, bias, h0, lengths});
     if (wants_grad({x, w, bias, h0})) return ShortConv::apply(x, w, opt(bias), opt(h0), opt(lengths), silu, want);
@@ -234,6 +239,7 @@ Tensor short_conv_step(const Tensor& x_, const Tensor& state, const Tensor& weig
     const int64_t B = x_.size(0), D = x_.size(1), K = weight.size(1);
     const Tensor x = seq(what, "x", x_, x_.sizes(), std::nullopt), w = f32(what, "weight", weight, {D, K}), bias = f32(what, "bias", bias_, {D});
     in_place(what, state, {B, K - 1, D});
+    not_traced(what);
     no_tangents(what, {x, w, bias, state});
     same_gpu(what, x, {w, bias, state});
     TORCH_CHECK(!wants_grad({x, w, bias, state}), what, " has no gradient: call it under torch.no_grad()");
@@ -361,6 +367,7 @@ variable_list ssm_scan(const Tensor& x, const Tensor& dt, const Tensor& a, const
     TORCH_CHECK_VALUE(x.dim() == 3, what, ": x must be a tensor (B, T, D)");
     const ScanArgs r = scan_args(what, x, dt, a, b, c, skip, gate, dt_bias);
     const Tensor h0 = f32(what, "initial_state", state_, {x.size(0), x.size(2), a.size(1)}), lengths = int_lengths(what, lengths_, x.size(0));
+    not_traced(what);
     no_tangents(what, {r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0});
     same_gpu(what, r.x, {r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0, lengths});
     if (wants_grad({r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0}))
@@ -374,6 +381,7 @@ Tensor ssm_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor
     TORCH_CHECK_VALUE(x.dim() == 2, what, ": x must be a tensor (B, D)");
     const ScanArgs r = scan_args(what, x, dt, a, b, c, skip, gate, dt_bias);
     in_place(what, state, {x.size(0), x.size(1), a.size(1)});
+    not_traced(what);
     no_tangents(what, {r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state});
     same_gpu(what, r.x, {r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state});
     TORCH_CHECK(!wants_grad({r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state}), what, " has no gradient: call it under torch.no_grad()");
