@@ -621,3 +621,14 @@ def test_forward_mode_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, fwd.make_dual(s["dy"], torch.ones_like(s["dy"])), retain_graph=True)
             torch.autograd.grad(y, leaf, s["dy"])
+
+
+def test_gradients_with_their_sign_put_off():
+    """The outputs' and the states' gradients as contiguous negative views."""
+    s, k = _scan_case(52, 2, 20, 70, 8, 1, "fp32"), _conv_case(53, 2, 20, 70, 4, "fp32")
+    for run, c in ((_scan_run, s), (_conv_run, k)):
+        v = dict(c, dy=torch._neg_view(c["dy"]), dh=torch._neg_view(c["dh"]))
+        want = run(dict(c, dy=-c["dy"], dh=-c["dh"]))
+        assert v["dh"].is_contiguous() and v["dh"].is_neg()
+        got = run(v)
+        assert all(torch.equal(got[n], want[n]) for n in want)

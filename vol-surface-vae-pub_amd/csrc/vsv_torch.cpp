@@ -194,7 +194,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
             at::NoGradGuard no_grad;
             c10::DeviceGuard guard(x.device());
             dy = dy.defined() ? last_contiguous(dy) : at::zeros_like(x, x.options(), at::MemoryFormat::Contiguous);
-            if (dstate.defined()) dstate = dstate.contiguous();
+            if (dstate.defined()) dstate = dstate.resolve_neg().contiguous();
             dx = whole_like(x);
             dw = grad_like(w);
             db = grad_like(bias);
@@ -342,7 +342,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
             at::NoGradGuard no_grad;
             c10::DeviceGuard guard(r.x.device());
             dy = dy.defined() ? last_contiguous(dy) : at::zeros_like(r.x, r.x.options(), at::MemoryFormat::Contiguous);
-            if (dstate.defined()) dstate = dstate.contiguous();
+            if (dstate.defined()) dstate = dstate.resolve_neg().contiguous();
             dx = whole_like(r.x); ddt = whole_like(r.x); db = whole_like(r.b); dc = whole_like(r.c);
             if (r.gate.defined()) dgate = whole_like(r.x);
             da = grad_like(r.a); dskip = grad_like(r.skip); dbias = grad_like(r.dt_bias); dh = grad_like(h0);
