@@ -632,3 +632,34 @@ def test_gradients_with_their_sign_put_off():
         assert v["dh"].is_contiguous() and v["dh"].is_neg()
         got = run(v)
         assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("T, N", [(64, 4), (2048, 4), (100, 16), (1100, 16), (300, 8)])
+def test_scan_states_that_grow(T, N):
+    """Decays whose product over a segment of time leaves float32, over states (backwards: gradients) that are zero there: inputs in
+    the last three steps only, the outputs' gradients in the first three."""
+    s = _scan_case(54, 2, T, 5, N, 1, "fp32", "s")
+    s["a"] = torch.full_like(s["a"], 8.0)                                    # (two tiles of steps of 1: e^128)
+    s["dt"] = torch.ones_like(s["dt"])
+    s["x"][:, :-3] = 0.0
+    s["dy"][:, 3:] = 0.0
+    s["dh"].zero_()
+    _scan_check(s, _scan_run(s, softplus=False), softplus=False)
+
+
+@pytest.mark.parametrize("T", [64, 2048])
+def test_scan_small_states_that_grow(T):
+    """A state of 1e-30 and a state's gradient of the same size, past 1e43 times that in one segment of time, no further."""
+    for first in (True, False):
+        s = _scan_case(55, 2, T, 5, 4, 1, "fp32", "sh")
+        s["a"] = torch.full_like(s["a"], 100.0 / 16.0)
+        s["dt"] = torch.zeros_like(s["dt"])
+        s["dt"][:, :16 if first else T] = 1.0
+        if not first:
+            s["dt"][:, :T - 16] = 0.0
+        s["x"].zero_()
+        s["dy"].zero_()
+        s["h0"] *= 1e-30 if first else 0.0
+        s["dh"] *= 0.0 if first else 1e-30
+        # (the exponent 16 x 6.25 log2 e = 144 is rounded three times: 3 x 100 half steps, within the 8 T + 64 of the bound)
+        _scan_check(s, _scan_run(s, softplus=False), softplus=False)

@@ -1,6 +1,8 @@
 // Selective state space memory: the short causal convolution, the scan, their backward passes and their single-token
 // forms.  Rows are (sequence, time step), features are contiguous; states, statistics and parameter gradients are
 // float32 whatever the sequences' type.
+#include <cfloat>
+
 #include "vsv_ops.h"
 
 namespace vsv {
@@ -530,6 +532,17 @@ template <int P> __device__ inline void sums_to_own(const float (&all)[kTile], f
     }
 }
 
+// w v + e, w = 2^x.  Where w leaves float32 (states that grow), a v of 0 stays 0 and one that is small enough takes w in two halves.
+__device__ inline float carry_on(float x, float w, float v, float e) {
+    float r = __builtin_fmaf(w, v, e);
+    if (w > FLT_MAX) {
+        asm volatile("");                                                 // (a branch: not taken by states that decay)
+        const float half = exp2_fast(0.5f * x);
+        r = v == 0.0f ? e : __builtin_fmaf(v * half, half, e);
+    }
+    return r;
+}
+
 // v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to; the loads of kAhead of them are
 // under way at a time.
 template <int R>
@@ -557,7 +570,7 @@ __device__ inline void fold_segments(const float* E, const float* sd, long row_f
             float w[R];
             decays<R>(s[u], A2, w);
 #pragma unroll
-            for (int m = 0; m < R; ++m) v[m] = __builtin_fmaf(w[m], v[m], e[u][m]);
+            for (int m = 0; m < R; ++m) v[m] = carry_on(s[u] * A2[m], w[m], v[m], e[u][m]);
         }
     }
 }
@@ -589,7 +602,8 @@ __global__ void __launch_bounds__(64) ssm_join_kernel(const float* __restrict__ 
         for (int u = 0; u < kAhead; ++u) {
             if (i + u >= S) break;
             E[(b * S + (back ? S - 1 - i - u : i + u)) * R * D + at] = v;
-            v = __builtin_fmaf(exp2_fast(s[u] * A2), v, e[u]);
+            const float x = s[u] * A2;
+            v = carry_on(x, exp2_fast(x), v, e[u]);
         }
     }
 }
