@@ -663,3 +663,16 @@ def test_scan_small_states_that_grow(T):
         s["dh"] *= 0.0 if first else 1e-30
         # (the exponent 16 x 6.25 log2 e = 144 is rounded three times: 3 x 100 half steps, within the 8 T + 64 of the bound)
         _scan_check(s, _scan_run(s, softplus=False), softplus=False)
+
+
+@pytest.mark.parametrize("a", [float("-inf"), -3e38])
+@pytest.mark.parametrize("T, N", [(5, 4), (5, 16), (100, 16), (300, 3), (2100, 4)])
+def test_scan_states_that_are_forgotten_at_once(T, N, a):
+    """a = -inf, and an a whose exponent leaves float32: padding, behind a length or in a last tile, leaves the state alone.  The values
+    and gradients are those of a = -1e30, whose decays are 0 too (as an infinity the formula's gradient would be 0 times it)."""
+    s = _scan_case(56, 3, T, 6, N, 1, "fp32", "sgh")
+    n = torch.tensor([T, T // 2, 0], dtype=torch.int32).cuda()
+    s["a"][:, 0] = a
+    got = _scan_run(s, n)
+    s["a"][:, 0] = -1e30
+    _scan_check(s, got, n)

@@ -487,9 +487,15 @@ template <int R> __device__ inline void store_states(float* p, long D, long d, c
 
 __device__ inline int tile_left(const ScanPos& p, long t) { return p.t1 - t < kTile ? (int)(p.t1 - t) : kTile; }
 
+// a log2 e.  A state that is forgotten at once (a = -inf, or below what float32 holds of the product) stays finite here: padding's
+// delta of 0 must leave it as it is, and 0 times infinity would not.
+__device__ inline float decay_exponent(float a) {
+    const float x = a * kLog2e;
+    return x < -FLT_MAX ? -FLT_MAX : x;
+}
 template <int R> __device__ inline void load_decay(const vsv_ssm_desc& a, long d, float (&A2)[R], int n0 = 0) {
 #pragma unroll
-    for (int n = 0; n < R; ++n) A2[n] = n0 + n < a.N ? a.a[d * a.N + n0 + n] * kLog2e : 0.0f;
+    for (int n = 0; n < R; ++n) A2[n] = n0 + n < a.N ? decay_exponent(a.a[d * a.N + n0 + n]) : 0.0f;
 }
 
 // Between the P lanes of a channel, 64 / P apart, of which lane `part` owns steps part kTile / P + j of a tile: values of the
@@ -585,7 +591,7 @@ __global__ void __launch_bounds__(64) ssm_join_kernel(const float* __restrict__ 
     if (id >= rows * R * D) return;
     const long b = id / (R * D), at = id - b * R * D, k = at / (4 * D), d = (at - k * 4 * D) >> 2;
     const int n = (int)(k * 4 + (at & 3));
-    const float A2 = n < N ? a[d * N + n] * kLog2e : 0.0f;
+    const float A2 = n < N ? decay_exponent(a[d * N + n]) : 0.0f;
     float v = n < N && init ? init[(b * D + d) * N + n] : 0.0f;
     for (int i = 0; i < S; i += kAhead) {
         float e[kAhead], s[kAhead];
