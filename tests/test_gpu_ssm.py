@@ -676,3 +676,30 @@ def test_scan_states_that_are_forgotten_at_once(T, N, a):
     got = _scan_run(s, n)
     s["a"][:, 0] = -1e30
     _scan_check(s, got, n)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_memory_whatever_its_padding_holds(kind):
+    """Outputs, states and every gradient as with zeros there; lengths outside [0, T] count as the nearest of the two."""
+    from vsv.ssm import SsmMemory
+    torch.manual_seed(3)
+    mem = SsmMemory(6, 20).cuda()
+    x, dy = torch.randn(4, 11, 6, device="cuda"), torch.randn(4, 11, 20, device="cuda")
+    n = torch.tensor([11, 4, 0, 900], dtype=kind, device="cuda")
+    pad = torch.arange(11, device="cuda") >= n[:, None]
+    got = []
+    for fill in (0.0, float("nan"), float("inf")):
+        mem.zero_grad()
+        leaf = x.clone()
+        leaf[pad] = fill
+        leaf.requires_grad_(True)
+        y, state = mem(leaf, lengths=n)
+        (y * dy).sum().backward()
+        got.append([y.detach(), *(t.detach() for t in state), leaf.grad, *(p.grad.clone() for p in mem.parameters())])
+    assert all(torch.isfinite(t).all() for t in got[0]) and (got[0][3][pad] == 0).all()
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    with pytest.raises(ValueError, match="lengths"):
+        mem(x, lengths=[11, 4, 0, 11])
+    with pytest.raises(ValueError, match="tensors are on"):
+        mem(x, lengths=n.cpu())

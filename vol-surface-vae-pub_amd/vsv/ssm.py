@@ -80,12 +80,20 @@ def ssm_step(x, dt, a, b, c, skip=None, gate=None, *, state, dt_bias=None, softp
         raise _not_a_tensor("ssm_step", e, dict(x=x, dt=dt, a=a, b=b, c=c, skip=skip, gate=gate, state=state, dt_bias=dt_bias)) from None
 
 
+def _padding_cleared(x, lengths):
+    """Zeros behind every row's length: a projection reads those rows, and its weights' gradient would be 0 times what they hold."""
+    if not isinstance(lengths, torch.Tensor) or lengths.shape != x.shape[:1] or lengths.device != x.device:
+        return x                                                           # (none, or short_conv's to refuse)
+    padding = torch.arange(x.shape[1], device=x.device) >= lengths[:, None]
+    return x.masked_fill(padding.unsqueeze(-1), 0.0)
+
+
 # ---- the memory they make up -------------------------------------------------------------------------------------
 
 class SsmMemory(torch.nn.Module):
     """A sequence memory called as nn.LSTM(batch_first=True) is: forward(x (B, T, input_size), state=None, lengths=None) ->
     (y (B, T, hidden_size), state), state = (the convolution's (B, taps - 1, hidden_size), the scan's
-    (B, hidden_size, state_size)).  step(x (B, input_size), state) takes one new token and updates the state in place."""
+    (B, hidden_size, state_size)); rows behind a length may hold anything.  step(x (B, input_size), state) takes one new token and updates the state in place."""
 
     def __init__(self, input_size, hidden_size, state_size=16, taps=4, dt_rank=None):
         super().__init__()
@@ -110,7 +118,7 @@ class SsmMemory(torch.nn.Module):
         return self.dt_proj(dt), b, c
 
     def forward(self, x, state=None, lengths=None):
-        x, gate = self.in_proj(x).chunk(2, dim=-1)
+        x, gate = self.in_proj(_padding_cleared(x, lengths)).chunk(2, dim=-1)
         conv, scan = state if state is not None else (None, None)
         x, conv = short_conv(x, self.conv_weight.float(), self.conv_bias.float(), initial_state=conv, lengths=lengths, return_state=True)
         dt, b, c = self._projected(x)
