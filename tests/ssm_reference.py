@@ -101,6 +101,31 @@ def scan_ref(x, dt, a, b, c, skip, gate, dt_bias, h0, lengths, softplus=True, dy
     return out
 
 
+def scan_plan(B, T, D, N, G, forward=True):
+    """(lanes that share a channel, segments, whether a launch of its own joins them) of a scan: the launcher's rule, with which
+    kernels a size runs.  One lane: ssm_ends_kernel and ssm_scan_kernel, more: ssm_shared_kernel; joined: ssm_join_kernel."""
+    R = 4 if N <= 4 else 8 if N <= 8 else 16
+    waves, tiles, S, P = B * G * -(-(D // G) // 64), -(-T // 8), 1, 1
+    if 0 < waves < 512:
+        if forward and N > 4 and (T < 64 or waves * tiles <= 6144):
+            P = R // 4
+        if T >= (64 if P > 1 else 40):
+            S = min(-(-2048 // (waves * P)), tiles // 2, 256)
+    S = -(-tiles // -(-tiles // S)) if tiles else 1
+    return P, S, S >= 24
+
+
+# (B, T, D, N, G) -> what of it: every way that a forward pass of 5 to 16 states is divided, for either padded number of states
+SCAN_PLANS = {
+    (7, 41, 70, 16, 1): "shared", (7, 41, 70, 8, 1): "shared",
+    (60, 130, 40, 13, 1): "shared split", (60, 130, 40, 6, 2): "shared split",
+    (3, 700, 66, 16, 1): "shared joined", (3, 700, 66, 8, 2): "shared joined",
+    (520, 20, 40, 16, 1): "alone", (260, 21, 130, 13, 1): "alone", (520, 20, 40, 8, 1): "alone", (515, 75, 24, 9, 2): "alone",
+    (400, 131, 24, 16, 1): "alone split", (200, 250, 70, 5, 1): "alone split",
+    (80, 620, 24, 16, 1): "alone joined", (40, 617, 70, 11, 1): "alone joined", (40, 620, 70, 8, 1): "alone joined",
+}
+
+
 def check(name, got, want, size, k):
     """|got - want| <= half a step of got's type at want + k half steps of float32 at the terms' size."""
     got, dtype = got.detach(), got.dtype

@@ -8,7 +8,7 @@ products and sums, the activation and its slope fewer than 32; sums over time an
 import pytest
 import torch
 
-from ssm_reference import check, conv_ref, scan_ref
+from ssm_reference import SCAN_PLANS, check, conv_ref, scan_ref
 
 pytestmark = pytest.mark.gpu
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
@@ -703,3 +703,32 @@ def test_memory_whatever_its_padding_holds(kind):
         mem(x, lengths=[11, 4, 0, 11])
     with pytest.raises(ValueError, match="tensors are on"):
         mem(x, lengths=n.cpu())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", list(SCAN_PLANS), ids=lambda s: SCAN_PLANS[s].replace(" ", "-") + "-" + "x".join(map(str, s)))
+def test_scan_however_it_is_divided(shape, dtype):
+    """Every kernel that a forward pass can take, elementwise, with lengths, a carried state and every gradient."""
+    s = _scan_case(57, *shape, dtype)
+    B, T = shape[:2]
+    n = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(58), dtype=torch.int32)
+    n[0], n[1], n[2] = T, 0, T - 1
+    n = n.cuda()
+    s["x"][torch.arange(T).cuda()[None, :] >= n[:, None]] = float("nan")
+    _scan_check(s, _scan_run(s, n), n)
+
+
+@pytest.mark.parametrize("B, T, D, dtype", [(64, 1000, 1024, "bf16"), (64, 2100, 1024, "fp16"), (64, 1000, 1024, "fp32"), (64, 500, 515, "fp32"),
+                                            (64, 1010, 515, "bf16")])
+def test_conv_in_long_chunks(B, T, D, dtype):
+    """Chunks of 32 and 64 rows forward, 128 backward (threads: 524288 and 131072 at least, of four channels each or of one): 40 channels, the
+    first and the last among them, elementwise with their gradients; lengths that end anywhere in a chunk."""
+    s = _conv_case(59, B, T, D, 4, dtype)
+    g = torch.Generator().manual_seed(60)
+    n = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32)
+    n[:4] = torch.tensor([T, T - 1, 64, 127], dtype=torch.int32)
+    n = n.cuda()
+    got = _conv_run(s, n)
+    at = torch.cat([torch.tensor([0, D - 1]), torch.randperm(D, generator=g)[:38]]).cuda()
+    part = {k: v[:, :, at] if k in ("x", "h0", "dy", "dh") else v[at] for k, v in s.items()}
+    _conv_check(part, {k: v[at] if k in ("w", "bias") else v[:, :, at] for k, v in got.items()}, n)

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from ssm_reference import conv_ref, scan_ref
+from ssm_reference import SCAN_PLANS, conv_ref, scan_plan, scan_ref
 
 
 def _case(seed, B=2, T=5, D=4, N=3, G=2, K=3):
@@ -288,6 +288,22 @@ def test_hooks_of_load_state_dict():
     opt.register_load_state_dict_pre_hook(lambda _, d: {**d, "state": {0: {**d["state"][0], "exp_avg": torch.zeros(5)}}})
     with pytest.raises(ValueError, match="exp_avg"):
         opt.load_state_dict(saved)
+
+
+def test_scan_sizes_reach_every_plan():
+    """The sizes that the GPU tests take run the kernels they name: the plan written again agrees with the workspace that the
+    library asks for (B S (padded states + 1) D floats of a scan in S > 1 segments), and each of the ways is there."""
+    from vsv import lib as vlib
+    L = vlib.load()
+    seen = set()
+    for (B, T, D, N, G), what in SCAN_PLANS.items():
+        P, S, joined = scan_plan(B, T, D, N, G)
+        assert what == ("shared" if P > 1 else "alone") + (" joined" if joined else " split" if S > 1 else ""), (B, T, D, N, G, P, S)
+        R = 8 if N <= 8 else 16
+        seen.add((R, what))
+        d = vlib.VsvSsm(dtype=0, N=N, softplus=1, B=B, T=T, D=D, G=G, x=16, dt=16, b=16, c=16, a=16, y=16)
+        assert L.vsv_ssm_scan_ws_bytes(C.byref(d)) == (4 * B * S * (R + 1) * D if S > 1 else 0), (B, T, D, N, G)
+    assert seen == {(R, lanes + how) for R in (8, 16) for lanes in ("shared", "alone") for how in ("", " split", " joined")}
 
 
 def test_c_entries_check_their_arguments():
