@@ -5,6 +5,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -116,10 +117,14 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     return false;
 }
 
-// A tangent would be dropped without a word: what follows looks at requires_grad and at memory alone.
-void no_tangents(const char* what, std::initializer_list<Tensor> ts) {
-    for (const Tensor& t : ts)
+// A tangent would be dropped without a word: what follows looks at requires_grad and at memory alone.  (No level, no tangents:
+// the usual call asks once, as a question to every tensor took the host 0.5 us a call.)
+template <typename... Ts> void no_tangents(const char* what, const Ts&... ts) {
+    if (!torch::autograd::ForwardADLevel::try_get_by_idx(0)) return;
+    auto one = [&](const Tensor& t) {
         TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative, and an input carries a tangent");
+    };
+    (one(ts), ...);
 }
 
 // A tracer sees none of the calls below: it would keep this call's outputs as constants.
@@ -188,7 +193,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
         const Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &h0 = saved[3], &lengths = saved[4];
         Tensor dy = grads[0], dstate = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !dstate.defined()) return variable_list(7);
-        no_tangents("short_conv's backward pass", {dy, dstate});
+        no_tangents("short_conv's backward pass", dy, dstate);
         Tensor dx, dw, db, dh;
         {
             at::NoGradGuard no_grad;
@@ -226,7 +231,7 @@ variable_list short_conv(const Tensor& x_, const Tensor& weight, const OptTensor
     const Tensor w = f32(what, "weight", weight, {D, K}), bias = f32(what, "bias", bias_, {D}), h0 = f32(what, "initial_state", state_, {B, K - 1, D});
     const Tensor lengths = int_lengths(what, lengths_, B);
     not_traced(what);
-    no_tangents(what, {x, w, bias, h0});
+    no_tangents(what, x, w, bias, h0);
     same_gpu(what, x, {w, bias, h0, lengths});
     if (wants_grad({x, w, bias, h0})) return ShortConv::apply(x, w, opt(bias), opt(h0), opt(lengths), silu, want);
     return conv_forward(x, w, bias, h0, lengths, silu, want);
@@ -240,7 +245,7 @@ Tensor short_conv_step(const Tensor& x_, const Tensor& state, const Tensor& weig
     const Tensor x = seq(what, "x", x_, x_.sizes(), std::nullopt), w = f32(what, "weight", weight, {D, K}), bias = f32(what, "bias", bias_, {D});
     in_place(what, state, {B, K - 1, D});
     not_traced(what);
-    no_tangents(what, {x, w, bias, state});
+    no_tangents(what, x, w, bias, state);
     same_gpu(what, x, {w, bias, state});
     TORCH_CHECK(!wants_grad({x, w, bias, state}), what, " has no gradient: call it under torch.no_grad()");
     c10::DeviceGuard guard(x.device());
@@ -336,7 +341,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
         const Tensor &h0 = s[8], &lengths = s[9], &saved = s[10];
         Tensor dy = grads[0], dstate = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !dstate.defined()) return variable_list(12);
-        no_tangents("ssm_scan's backward pass", {dy, dstate});
+        no_tangents("ssm_scan's backward pass", dy, dstate);
         Tensor dx, ddt, dgate, db, dc, da, dskip, dbias, dh;
         {
             at::NoGradGuard no_grad;
@@ -368,7 +373,7 @@ variable_list ssm_scan(const Tensor& x, const Tensor& dt, const Tensor& a, const
     const ScanArgs r = scan_args(what, x, dt, a, b, c, skip, gate, dt_bias);
     const Tensor h0 = f32(what, "initial_state", state_, {x.size(0), x.size(2), a.size(1)}), lengths = int_lengths(what, lengths_, x.size(0));
     not_traced(what);
-    no_tangents(what, {r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0});
+    no_tangents(what, r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0);
     same_gpu(what, r.x, {r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0, lengths});
     if (wants_grad({r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, h0}))
         return SsmScan::apply(r.x, r.dt, r.a, r.b, r.c, opt(r.skip), opt(r.gate), opt(r.dt_bias), opt(h0), opt(lengths), softplus, want);
@@ -382,7 +387,7 @@ Tensor ssm_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor
     const ScanArgs r = scan_args(what, x, dt, a, b, c, skip, gate, dt_bias);
     in_place(what, state, {x.size(0), x.size(1), a.size(1)});
     not_traced(what);
-    no_tangents(what, {r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state});
+    no_tangents(what, r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state);
     same_gpu(what, r.x, {r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state});
     TORCH_CHECK(!wants_grad({r.x, r.dt, r.a, r.b, r.c, r.skip, r.gate, r.dt_bias, state}), what, " has no gradient: call it under torch.no_grad()");
     c10::DeviceGuard guard(r.x.device());
