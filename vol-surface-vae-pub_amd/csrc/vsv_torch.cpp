@@ -4,6 +4,7 @@
 // The C entries' addresses come from the library that vsv/lib.py has loaded (bind), so there is one copy of it.
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -416,6 +417,11 @@ void apart(std::vector<std::pair<uintptr_t, uintptr_t>>& spans) {
         TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "AdamW: two parameters share memory");
 }
 
+void refuse_capture() {                                                    // of the current device's current stream
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "AdamW.step cannot be captured into a HIP graph: the step count is a launch argument");
+}
+
 void adamw_step(int bits, std::vector<AdamwCall> calls) {
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     for (auto& [p, g, m, v, ms, vs, lr, b1, b2, eps, wd, step] : calls) {   // everything is checked before anything is launched
@@ -435,6 +441,14 @@ void adamw_step(int bits, std::vector<AdamwCall> calls) {
         }
     }
     apart(spans);
+    at::Device asked(at::kCPU);
+    for (const auto& call : calls)
+        for (const Tensor& p : std::get<0>(call)) {
+            if (!p.is_cuda() || p.device() == asked) continue;
+            asked = p.device();
+            c10::DeviceGuard guard(asked);
+            refuse_capture();
+        }
     for (auto& call : calls) {
         auto& [p, g, m, v, ms, vs, lr, b1, b2, eps, wd, step] = call;
         for (size_t i = 0; i < p.size(); ++i) {
@@ -491,5 +505,6 @@ PYBIND11_MODULE(_vsv_torch, m) {
     m.def("ssm_scan", &ssm_scan);
     m.def("ssm_step", &ssm_step);
     m.def("adamw_step", &adamw_step);
+    m.def("refuse_capture", &refuse_capture);
     m.def("adamw_read8", &adamw_read8);
 }

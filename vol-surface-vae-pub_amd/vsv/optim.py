@@ -59,6 +59,9 @@ class AdamW(torch.optim.Optimizer):
                 "exp_avg_scale": (blocks, torch.float32), "exp_avg_sq_scale": (blocks, torch.float32)}
 
     def _init_state(self, p):
+        if p.is_cuda:                                                      # (under capture the zeros would only be recorded)
+            with torch.cuda.device(p.device):
+                _native.load().refuse_capture()
         self.state[p] = {"step": 0, **{k: torch.zeros(shape, dtype=dtype, device=p.device) for k, (shape, dtype) in self._layout(p).items()}}
         return self.state[p]
 
@@ -68,10 +71,6 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # (before any state is made: under capture its zeros would only be recorded)
-        for index in {p.get_device() for group in self.param_groups for p in group["params"] if p.grad is not None}:
-            if index >= 0 and _capturing(index):
-                raise RuntimeError("AdamW.step cannot be captured into a HIP graph: the step count is a launch argument")
         state, calls, states = self.state, [], []
         wide = self.state_bits == 32
         for group in self.param_groups:
@@ -79,7 +78,7 @@ class AdamW(torch.optim.Optimizer):
             for p in group["params"]:
                 g = p.grad
                 if g is not None:
-                    st = state[p] or self._init_state(p)
+                    st = state.get(p) or self._init_state(p)
                     rows.setdefault(st["step"], []).append((p, g, st))
             b1, b2 = group["betas"]
             for step, part in rows.items():
@@ -139,11 +138,6 @@ class AdamW(torch.optim.Optimizer):
                 # (torch's own optimizers keep the step count in a tensor: here it groups the parameters, and is a launch argument)
                 self.state[p] = {k: int(v) if k == "step" else v.detach().to(device=p.device, copy=True).contiguous()
                                  for k, v in st.items()}
-
-
-def _capturing(index):
-    with torch.cuda.device(index):
-        return torch.cuda.is_current_stream_capturing()
 
 
 def _check_options(group):
