@@ -2,6 +2,7 @@
 // forms.  Rows are (sequence, time step), features are contiguous; states, statistics and parameter gradients are
 // float32 whatever the sequences' type.
 #include <cfloat>
+#include <type_traits>
 
 #include "vsv_ops.h"
 
@@ -538,24 +539,23 @@ template <int P> __device__ inline void sums_to_own(const float (&all)[kTile], f
     }
 }
 
-// w v + e, w = 2^x.  Where w leaves float32 (states that grow), a v of 0 stays 0 and one that is small enough takes w in two halves.
-__device__ inline float carry_on(float x, float w, float v, float e) {
-    float r = __builtin_fmaf(w, v, e);
-    if (w > FLT_MAX) {
-        asm volatile("");                                                 // (a branch: not taken by states that decay)
-        const float half = exp2_fast(0.5f * x);
-        r = v == 0.0f ? e : __builtin_fmaf(v * half, half, e);
-    }
-    return r;
+// 2^x v + e where 2^x may leave float32 (states that grow): a v of 0 stays 0, any other takes the factor in two halves.
+__device__ inline float carry_past(float x, float v, float e) {
+    const float half = exp2_fast(0.5f * x);
+    return v == 0.0f ? e : __builtin_fmaf(v * half, half, e);
 }
 
-// v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to; the loads of kAhead of them are
-// under way at a time.
-template <int R>
+// v = exp(a sum delta) v + E over the segments from, from + step, .. up to (not including) to, from v = first(); the loads of
+// kAhead of them are under way at a time.  Should a factor of any lane leave float32, all of it once more, one segment at a time.  (A
+// branch in the loop itself costs ssm_scan_kernel a third of its waves, in registers; one that the lanes take apart costs ssm_bwd_kernel
+// 20 us of 270, in scalar registers that leave its loop for lanes of vector registers.)
+template <int R, typename F>
 __device__ inline void fold_segments(const float* E, const float* sd, long row_floats, long D, long d, long row0, int from, int to, int step,
-                                     const float (&A2)[R], float (&v)[R]) {
+                                     const float (&A2)[R], float (&v)[R], int N, F&& first) {
     constexpr int kAhead = 4;
     const int n = (to - from) * step;
+    float top = 0.0f;
+    first(v, N);
     for (int i = 0; i < n; i += kAhead) {
         float e[kAhead][R], s[kAhead];
 #pragma unroll
@@ -576,8 +576,25 @@ __device__ inline void fold_segments(const float* E, const float* sd, long row_f
             float w[R];
             decays<R>(s[u], A2, w);
 #pragma unroll
-            for (int m = 0; m < R; ++m) v[m] = carry_on(s[u] * A2[m], w[m], v[m], e[u][m]);
+            for (int m = 0; m < R; ++m) {
+                v[m] = __builtin_fmaf(w[m], v[m], e[u][m]);
+                top = __builtin_fmaxf(top, w[m]);
+            }
         }
+    }
+    if (!__any(top > FLT_MAX)) return;
+    int again = N;
+    asm volatile("" : "+s"(again));                                       // (or the first time's n < N are kept until here)
+    first(v, again);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const long k = row0 + from + i * step;
+        float e[R], w[R];
+        load_states<R>(E + k * row_floats, D, d, e);
+        const float s = sd[k * D + d];
+        decays<R>(s, A2, w);
+#pragma unroll
+        for (int m = 0; m < R; ++m) v[m] = w[m] > FLT_MAX ? carry_past(s * A2[m], v[m], e[m]) : __builtin_fmaf(w[m], v[m], e[m]);
     }
 }
 
@@ -604,13 +621,22 @@ __global__ void __launch_bounds__(64) ssm_join_kernel(const float* __restrict__ 
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) { pin(e[u]); pin(s[u]); }         // (all of them under way, none loaded behind the break)
+        float w[kAhead], top = 0.0f;
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (i + u >= S) break;
-            E[(b * S + (back ? S - 1 - i - u : i + u)) * R * D + at] = v;
-            const float x = s[u] * A2;
-            v = carry_on(x, exp2_fast(x), v, e[u]);
+            w[u] = exp2_fast(s[u] * A2);
+            top = __builtin_fmaxf(top, w[u]);
         }
+        auto take = [&](auto past) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (i + u >= S) break;
+                E[(b * S + (back ? S - 1 - i - u : i + u)) * R * D + at] = v;
+                v = past.value && w[u] > FLT_MAX ? carry_past(s[u] * A2, v, e[u]) : __builtin_fmaf(w[u], v, e[u]);
+            }
+        };
+        if (__any(top > FLT_MAX)) take(std::true_type{});
+        else take(std::false_type{});
     }
 }
 
@@ -684,10 +710,12 @@ __global__ void __launch_bounds__(64) ssm_scan_kernel(const vsv_ssm_desc a, cons
     if (p.t0 < p.t1) fetch(tile_left(p, p.t0));
     float A2[R], h[R];
     load_decay<R>(a, d, A2);
+    auto first = [&](float (&v)[R], int N) {
 #pragma unroll
-    for (int n = 0; n < R; ++n) h[n] = n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n] : 0.0f;
+        for (int n = 0; n < R; ++n) v[n] = n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n] : 0.0f;
+    };
     if (pl.joined) load_states<R>(E + (p.b * pl.S + p.s) * R * D, D, d, h);
-    else fold_segments<R>(E, sd, R * D, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
+    else fold_segments<R>(E, sd, R * D, D, d, p.b * pl.S, 0, p.s, 1, A2, h, N, first);
     const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     float* saved = a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D : nullptr;
     int buf = 0;
@@ -775,10 +803,13 @@ __global__ void __launch_bounds__(64) ssm_shared_kernel(const vsv_ssm_desc a, co
     float A2[L], h[L], sum = 0.0f;
     const long segment = (p.b * pl.S + p.s) * R * D + n0 * D;
     load_decay<L>(a, d, A2, n0);
+    auto first = [&](float (&v)[L], int N) {
 #pragma unroll
-    for (int n = 0; n < L; ++n) h[n] = !ENDS && n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
-    if (!ENDS && pl.joined) load_states<L>(E + segment, D, d, h);
-    else if (!ENDS) fold_segments<L>(E + n0 * D, sd, R * D, D, d, p.b * pl.S, 0, p.s, 1, A2, h);
+        for (int n = 0; n < L; ++n) v[n] = !ENDS && n0 + n < N && a.state_in ? a.state_in[(p.b * D + d) * N + n0 + n] : 0.0f;
+    };
+    if (ENDS) first(h, N);
+    else if (pl.joined) load_states<L>(E + segment, D, d, h);
+    else fold_segments<L>(E + n0 * D, sd, R * D, D, d, p.b * pl.S, 0, p.s, 1, A2, h, N, first);
     const float skip = a.skip ? a.skip[d] : 0.0f, dtb = a.dt_bias ? a.dt_bias[d] : 0.0f;
     float* saved = !ENDS && a.saved ? a.saved + (p.b * ((a.T + kTile - 1) / kTile) + p.t0 / kTile) * R * D + n0 * D : nullptr;
     int buf = 0;
@@ -961,10 +992,12 @@ __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, co
     const long bc_ts = a.G * 2 * R;
     float A2[R], q[R], dA[R] = {};
     load_decay<R>(a, d, A2);
+    auto first = [&](float (&v)[R], int N) {
 #pragma unroll
-    for (int n = 0; n < R; ++n) q[n] = n < N && gr.d_state_out ? gr.d_state_out[(p.b * D + d) * N + n] : 0.0f;
+        for (int n = 0; n < R; ++n) v[n] = n < N && gr.d_state_out ? gr.d_state_out[(p.b * D + d) * N + n] : 0.0f;
+    };
     if (pl.joined) load_states<R>(E + (p.b * pl.S + p.s) * R * D, D, d, q);
-    else fold_segments<R>(E, sd, R * D, D, d, p.b * pl.S, pl.S - 1, p.s, -1, A2, q);
+    else fold_segments<R>(E, sd, R * D, D, d, p.b * pl.S, pl.S - 1, p.s, -1, A2, q, N, first);
     if (!p.live) {
 #pragma unroll
         for (int n = 0; n < R; ++n) q[n] = 0.0f;
