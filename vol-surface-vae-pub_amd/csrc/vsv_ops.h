@@ -40,7 +40,8 @@ __device__ inline float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.0f +
 
 // log(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p(u) = 2 atanh(s), s = u / (2 + u) <= 1/3, as s P(s^2): an interpolation
 // of 2 atanh(s) / s at the Chebyshev nodes of s^2 in [0, 1/9], 4e-9 relative.  (log(1 + u) itself would lose the small
-// time steps: softplus(-7) = 9e-4 needs all 24 bits of u, of which 1 + u keeps 14.)
+// time steps: softplus(-7) = 9e-4 needs all 24 bits of u, of which 1 + u keeps 14.)  u has the rounding of its own argument,
+// relative to it 4.4e-7 at |x| = 7 and 1.9e-6 at 40.
 __device__ inline float softplus_f(float x) {
     const float u = exp2_fast(-__builtin_fabsf(x) * kLog2e);
     const float s = u * __builtin_amdgcn_rcpf(2.0f + u), z = s * s;

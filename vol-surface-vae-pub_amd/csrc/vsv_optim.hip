@@ -83,7 +83,8 @@ __global__ void __launch_bounds__(256) adamw32_kernel(const Table tab, const Hyp
 // additive (Weyl) sequence over steps and elements (for v, 1 - u).  Over steps u is spread evenly, so the rounding is
 // unbiased in time; to the nearest code, v would never move: beta2 = 0.999 changes it by 0.1 % a step, codes are at least
 // 1.6 % apart.  v > 0 never becomes 0, which would leave m without its divisor.
-//   168 M bf16 parameters: 417 to 461 us, the issue of 90 vector operations an element (2.4 GB at the copy rate: 350 us).
+//   168 M bf16 parameters: 417 to 461 us, the issue of 90 vector operations an element (its 10.06 bytes an element, 1.69 GB,
+// take 350 us at the copy rate).
 //   The moments are computed in 64 bits (full rate on this chip), and so is the choice of a code wherever float32 could
 // choose another: the codes are the definition's, not a rounding away from it.
 //   A gradient that is not finite leaves its element's moments alone and makes the parameter NaN: a NaN scale would take

@@ -37,7 +37,7 @@ __device__ inline float conv_silu(float s) {
 }
 
 // pre[t,d] = bias[d] + sum_k w[d,k] xs[t-K+1+k, d],  y = silu(pre) or pre; xs is x, continued into state_in before t = 0.
-// One read of x and one write of y (2K flops an element): bound by memory (8x2048x4096 bf16: 61 us, 4.4 TB/s).  A thread owns VEC
+// One read of x and one write of y (2K flops an element): bound by memory (8x2048x4096 bf16: 57 to 61 us, 4.4 to 4.7 TB/s).  A thread owns VEC
 // neighbouring channels and a chunk of time, so the window stays in registers and only K-1 rows per chunk are read twice; it
 // works on kRows rows at a time, with the next ones under way.
 template <typename T, int K, int VEC, int kRows> struct ConvRows {
@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(256) short_conv_kernel(const vsv_short_conv_de
 
 // ds = dy act'(pre) (pre computed again from x), dx[t] = sum_k w[k] ds[t+K-1-k], dw[k] = sum_t ds[t] xs[t-K+1+k],
 // dbias = sum_t ds.  The same chunks; a chunk reads K-1 rows beyond each end, its sums over time go to `part`
-// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.  8x2048x4096 bf16: 92 us, 4.4 TB/s.
+// (chunk, K + 1, D) and are joined in a fixed order by sum_conv_parts_kernel.  8x2048x4096 bf16: 90 us, 4.5 TB/s; 16x8192x515, a
+// channel a thread in accesses of two bytes: 232 us, 16x8192x516: 145.
 template <typename T, int K, int VEC, int kRows>
 __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_conv_desc a, const vsv_short_conv_grads g, long chunk, long n_chunk,
                                                              long n_vec, float* __restrict__ part) {
@@ -252,7 +253,9 @@ __global__ void __launch_bounds__(256) short_conv_bwd_kernel(const vsv_short_con
     store_vec<float, VEC>(p + (long)K * a.D, db);
 }
 
-// out_j = sum over rows of part (rows, M); element m = k * D + d goes to dw[d * K + k] or, k == K, to dbias[d].
+// out_j = sum over rows of part (rows, M); element m = k * D + d goes to dw[d * K + k] or, k == K, to dbias[d].  A workgroup has 64
+// columns and all rows: 5 us where the channels are many (8x2048x4096), but 87 beside the pass's own 88 for 8192 rows of 64 channels
+// (64x16384x64), bound by the latency of a walk eight loads deep.
 __global__ void __launch_bounds__(256) sum_conv_parts_kernel(const float* __restrict__ part, long rows, long D, int K,
                                                              float* __restrict__ dw, float* __restrict__ dbias) {
     __shared__ float red[4][64];
@@ -297,7 +300,8 @@ __global__ void __launch_bounds__(256) short_conv_step_kernel(const T* __restric
 // delta = softplus(dt + dt_bias),  h_t = exp(delta a) h_{t-1} + delta x b_t,  y = (c_t . h_t + skip x) silu(gate).
 // The decay belongs to (channel, state), so there is no matrix form: per state and step one exponential and four float32
 // operations, 24 cycles of a SIMD per 64 channels, against 8 bytes of traffic per channel and step in 16 bits.  Bound by
-// the vector units: 1x16384x2048 bf16 takes 261 us in all, of which the issue of its vector instructions is 227.
+// the vector units: 1x16384x2048 bf16 takes 268 us in all, of which the issue of its vector instructions is 227; 256x512x1024, which
+// is not split, 557 us (375 at 24 cycles a state).
 //   A lane owns a channel and its N states (padded to R) in registers (or four of them), a wave 64 channels of one group (or
 // 256 / R), which share b_t and c_t.  x, dt, gate, b and c of the next kTile steps are loaded while the present ones are
 // computed; the activations are taken for a tile at a time.
@@ -971,7 +975,7 @@ template <int NV> __device__ inline float wave_sums(float (&v)[NV]) {
 // A tile at a time from the state saved in front of it: its states are computed again into registers, then q runs through
 // them in reverse, four states at a time so that they fit.  The gradients of b and c are sums over channels: over the
 // wave's 64 here, over the channel blocks in ssm_sums_kernel; those of a, skip and dt_bias sums over time: here, and over
-// sequences and segments there too.  All in a fixed order.  4x2048x2048 bf16: 273 us, vector units at two waves a SIMD.
+// sequences and segments there too.  All in a fixed order.  4x2048x2048 bf16: 265 to 274 us, vector units at two waves a SIMD.
 template <typename T, int R>
 __global__ void __launch_bounds__(64, 2) ssm_bwd_kernel(const vsv_ssm_desc a, const vsv_ssm_grads gr, const ScanPlan pl, const float* __restrict__ E,
                                                         const float* __restrict__ sd, float* __restrict__ part_bc, float* __restrict__ part_p) {
@@ -1299,9 +1303,13 @@ long ssm_blocks(const vsv_ssm_desc* a) { return (a->D / a->G + 63) / 64; }
 // slower at 64x128x100 to 5x777x198), at most kMaxSegments (1x4096x256 forward and backward: 64 segments 173 us, 256 124).  A
 // few segments are folded by those behind them, many in a launch of their own (5x777x198, 48 segments, forward: 34 and 31 us;
 // 4x2048x2048, 16 segments, backward: 329 and 340).
-//   Forward, and as long as that leaves about a wave per SIMD, a channel's states are shared by R / 4 lanes (16x256x100: 21 us
-// with one lane a channel, 15; 1x1024x256: 25 and 18; 64x1024x100, which has twice as many waves: 74 and 96), and a sequence
-// that is short enough is not split at all (64x60x100: in one pass 12, in segments 13; 64x96x100: 17 and 16.5).
+//   Forward, below as many waves, a channel's states are shared by R / 4 lanes where the sequence is short or the work is little: below
+// 64 steps, or up to kShareTiles tiles over all waves.  (It is a bound on work, not on waves: sharing issues 1.4 times the
+// instructions, which costs nothing while SIMDs stand idle.  16x256x100: 21 us with one lane a channel, 15; 1x1024x256: 25 and 18;
+// 64x1024x100, 16384 tiles: 74 and 96, both of them split; from 64 steps on sharing was not measured without a split.)  A sequence that
+// is short enough is not split at all (64x60x100: in one pass 12, in segments 13; 64x96x100: 17 and 16.5).  From 512 waves on nothing is
+// split or shared: 8x512x4096, 512 waves on 1024 SIMDs, takes 195 us, of which 24 cycles a state are 94 on the SIMDs
+// that have a wave.
 constexpr long kMaxSegments = 256, kSplitFrom = 40, kJoinFrom = 24, kShareBelow = 64, kShareTiles = 6144, kSplitWaves = 2048;
 
 ScanPlan scan_plan(const vsv_ssm_desc* a, bool forward) {
